@@ -518,6 +518,98 @@ int mrs_splitter_next(mrs_splitter* sp, uint32_t* shift, uint32_t* bits, uint32_
 int mrs_splitter_feed(mrs_splitter* sp, const uint64_t* counts);
 int mrs_splitter_get(const mrs_splitter* sp, mrs_split_result* out);
 
+/* ---- rows ordered by a small integer key, and back: tokens routed to experts ---------------
+ * No counterpart in the reference.  A token is a row of `hidden` elements; each of its `topk` slots
+ * names one of `experts` keys.  The four steps are a partial stable sort of every row of scores
+ * (mrs_route_select), a stable sort of all slots by key (mrs_route_order), the move of the rows into
+ * that order (mrs_route_dispatch) and the weighted way back (mrs_route_combine), each with its
+ * gradient where it has one.  Slot i = token * topk + j throughout.  Every call only enqueues
+ * kernels on `stream` (no allocation, no memset, no synchronisation) and may be captured into a HIP
+ * graph; results do not depend on timing (no floating-point atomics).  Only mrs_route_order uses
+ * memory of the handle: calls of it on one handle, and replays of graphs that hold one, must not
+ * overlap in time.  Buffers need the alignment of their element, nothing more. */
+typedef struct mrs_route mrs_route;
+
+#define MRS_GATE_SOFTMAX 0 /* p[e] = exp(s[e]) / sum of exp(s) over the experts that take part      */
+#define MRS_GATE_SIGMOID 1 /* p[e] = 1 / (1 + exp(-s[e]))                                          */
+
+#define MRS_TYPE_F32 0
+#define MRS_TYPE_F16 1
+#define MRS_TYPE_BF16 2
+#define MRS_TYPE_8BIT 3 /* elements of one byte, moved unseen (mrs_route_dispatch only)            */
+
+#define MRS_ROUTE_MAX_EXPERTS 1024
+#define MRS_ROUTE_MAX_TOPK 32
+
+typedef struct mrs_route_desc {
+    uint64_t tokens;   /* most tokens of one call; tokens * topk + experts * align < 2^31          */
+    int32_t experts;   /* 1 .. MRS_ROUTE_MAX_EXPERTS                                              */
+    int32_t topk;      /* slots a token has, 1 .. MRS_ROUTE_MAX_TOPK; select: at most `experts`   */
+    int32_t align;     /* an expert's rows start at a multiple of this, 1 .. 1024                 */
+    int32_t gate;      /* MRS_GATE_*                                                             */
+    uint64_t capacity; /* most rows an expert takes, later slots are dropped; 0 = no limit        */
+    int32_t normalize; /* 1: a token's weights are divided by their sum                          */
+    float scale;       /* factor on every weight (after the division)                            */
+} mrs_route_desc;
+
+/* Device arrays of the caller that say where every slot's row is: written by mrs_route_order, read
+ * by the calls that move rows. */
+typedef struct mrs_route_map {
+    int32_t* row_of_slot; /* [tokens * topk]: the slot's row, or -1 (no such expert, or over capacity) */
+    int32_t* slot_of_row; /* [rows]: the row's slot, or -1                                         */
+    int32_t* counts;      /* [experts]: rows the expert has                                        */
+    int32_t* offsets;     /* [experts + 1]: where its segment starts; the last one is the end of all */
+    uint64_t rows;        /* rows of the expert-ordered buffers, at least mrs_route_max_rows       */
+} mrs_route_map;
+
+int mrs_route_create(mrs_context* ctx, const mrs_route_desc* desc, mrs_route** out);
+int mrs_route_destroy(mrs_route* route);
+/* Host only: the most rows the slots of `desc` can take,
+ * n + min(n, experts) * (align - 1) for n = tokens * topk, or what `capacity` limits it to. */
+int mrs_route_max_rows(const mrs_route_desc* desc, uint64_t* rows);
+/* ids[t, :] = the topk largest keys of row t in descending order, equal keys lowest expert first, where
+ * key[e] = f32(scores[t, e]) + bias[e] (one addition in 32 bits; bias may be NULL).  An expert takes
+ * part if its key is above -infinity (so a masked score, a masked bias or a NaN never does); where
+ * fewer than topk do, the remaining ids are -1 and their weights 0.  The bias steers the choice only:
+ * weights[t, j] = scale * q, q = p[id] or, normalized, p[id] / sum over the token's slots.  A score of
+ * +infinity is chosen first, but a softmax over it is NaN.  `scores` has `tokens` rows of `experts`
+ * elements of `type` (not MRS_TYPE_8BIT), ld_scores elements apart. */
+int mrs_route_select(mrs_route* route, uint64_t tokens, const void* scores_dev, uint64_t ld_scores, int32_t type,
+                     const float* bias_dev, int32_t* ids_dev, float* weights_dev, void* stream);
+/* scores_grad[t, e] = sum over j of weights_grad[t, j] * d weights[t, j] / d scores[t, e] for the ids
+ * given (mrs_route_select's; ids that are negative, too large or masked count for nothing; a repeated
+ * id is as many slots).  All `experts` elements of each row are written.  scores_grad must not overlap
+ * the inputs. */
+int mrs_route_select_backward(mrs_route* route, uint64_t tokens, const void* scores_dev, uint64_t ld_scores, int32_t type,
+                              const float* bias_dev, const int32_t* ids_dev, const float* weights_grad_dev,
+                              void* scores_grad_dev, uint64_t ld_scores_grad, void* stream);
+/* Stable counting sort of the slots by ids_dev[slot].  A slot is kept if its id lies in [0, experts) and
+ * fewer than `capacity` earlier slots have it; every array of `map` is written in full. */
+int mrs_route_order(mrs_route* route, uint64_t tokens, const int32_t* ids_dev, const mrs_route_map* map, void* stream);
+/* rows[row_of_slot[t, j]] = x[t]; rows of a segment that no slot has (they fill it up to `align`) are
+ * zeroed, rows from offsets[experts] on are left as they are.  Indices outside [0, map->rows) are
+ * passed over, here and below.  x: `tokens` rows ld_x elements apart; rows: map->rows rows ld_rows
+ * apart; the two must not overlap. */
+int mrs_route_dispatch(mrs_route* route, uint64_t tokens, const mrs_route_map* map, int32_t type, uint64_t hidden,
+                       const void* x_dev, uint64_t ld_x, void* rows_dev, uint64_t ld_rows, void* stream);
+/* x_grad[t] = sum over j of rows_grad[row_of_slot[t, j]], in 32 bits in the order of j, rounded once;
+ * zeros for a token without rows. */
+int mrs_route_dispatch_backward(mrs_route* route, uint64_t tokens, const mrs_route_map* map, int32_t type, uint64_t hidden,
+                                const void* rows_grad_dev, uint64_t ld_rows_grad, void* x_grad_dev, uint64_t ld_x_grad,
+                                void* stream);
+/* out[t] = sum over j of weights[t, j] * rows[row_of_slot[t, j]], in 32 bits in the order of j, rounded
+ * once.  A slot without a row is left out whatever its weight; a token without rows gives zeros. */
+int mrs_route_combine(mrs_route* route, uint64_t tokens, const mrs_route_map* map, int32_t type, uint64_t hidden,
+                      const void* rows_dev, uint64_t ld_rows, const float* weights_dev, void* out_dev, uint64_t ld_out,
+                      void* stream);
+/* rows_grad[row_of_slot[t, j]] = weights[t, j] * out_grad[t] (rounded once; other rows as in
+ * mrs_route_dispatch) and weights_grad[t, j] = sum over h of out_grad[t, h] * rows[row_of_slot[t, j], h] in
+ * 32 bits, 0 for a slot without a row.  rows_grad must not overlap the inputs. */
+int mrs_route_combine_backward(mrs_route* route, uint64_t tokens, const mrs_route_map* map, int32_t type, uint64_t hidden,
+                               const void* out_grad_dev, uint64_t ld_out_grad, const void* rows_dev, uint64_t ld_rows,
+                               const float* weights_dev, void* rows_grad_dev, uint64_t ld_rows_grad, float* weights_grad_dev,
+                               void* stream);
+
 /* ---- input generator (stands in for create_scene's RNG, src/main.rs:114-161) */
 /* xyz_dev[3i+c] = top 24 bits of hash(seed, c, i) * 2^-24, uniform in [0,1). */
 int mrs_generate_points(mrs_context* ctx, uint64_t seed, uint64_t n, float* xyz_dev,

@@ -1,0 +1,148 @@
+"""Token routing without a GPU: the sizes the library reports, what it refuses, and that the definitions
+the GPU tests compare with have the derivatives they say."""
+import ctypes
+import types
+
+import pytest
+import torch
+
+import route_ref as ref
+import wgpu_morton_code_radix_sort_test_amd as mrs
+from wgpu_morton_code_radix_sort_test_amd import _lib
+
+
+def _desc(**kw):
+    d = dict(tokens=100, experts=8, topk=2, align=1, gate=0, capacity=0, normalize=1, scale=1.0)
+    d.update(kw)
+    return _lib.RouteDesc(*[d[name] for name, _ in _lib.RouteDesc._fields_])
+
+
+def _max_rows(**kw):
+    rows = ctypes.c_uint64()
+    return _lib.load_library().mrs_route_max_rows(ctypes.byref(_desc(**kw)), ctypes.byref(rows)), rows.value
+
+
+@pytest.mark.parametrize("tokens,experts,topk,align,capacity,want", [
+    (100, 8, 2, 1, 0, 200),
+    (100, 8, 2, 16, 0, 200 + 8 * 15),
+    (1, 256, 4, 16, 0, 4 + 4 * 15),  # only experts with a row need filling up
+    (0, 8, 2, 16, 0, 0),
+    (1000, 8, 2, 1, 10, 80),
+    (1000, 8, 2, 16, 10, 8 * 16),
+    (10, 8, 2, 1, 1000, 20),  # a capacity that limits nothing
+])
+def test_max_rows(tokens, experts, topk, align, capacity, want):
+    assert _max_rows(tokens=tokens, experts=experts, topk=topk, align=align, capacity=capacity) == (_lib.MRS_OK, want)
+
+
+def test_max_rows_holds_the_fullest_ordering():
+    g = torch.Generator().manual_seed(3)
+    for _ in range(50):
+        tokens, experts, topk = (int(torch.randint(1, hi, (1,), generator=g)) for hi in (40, 12, 6))
+        align, capacity = int(torch.randint(1, 9, (1,), generator=g)), int(torch.randint(0, 12, (1,), generator=g))
+        ids = torch.randint(-1, experts, (tokens, topk), generator=g)
+        rows = _max_rows(tokens=tokens, experts=experts, topk=topk, align=align, capacity=capacity)[1]
+        offsets = ref.order(ids, experts, align, capacity, 10000)[3]
+        assert int(offsets[-1]) <= rows
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(experts=0), "experts"), (dict(experts=1025), "experts"), (dict(topk=0), "topk"), (dict(topk=33), "topk"),
+    (dict(align=0), "align"), (dict(align=1025), "align"), (dict(gate=2), "gate"), (dict(normalize=2), "normalize"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(tokens=1 << 31), "tokens"),
+    (dict(tokens=1 << 30, topk=2), "tokens"), (dict(tokens=(1 << 64) - 1), "tokens"),
+])
+def test_bad_descriptions_are_refused(kw, word):
+    rc, _ = _max_rows(**kw)
+    assert rc == _lib.MRS_ERR_INVALID_ARGUMENT
+    assert word in _lib.load_library().mrs_last_error_string().decode()
+
+
+def test_null_arguments_are_refused():
+    lib = _lib.load_library()
+    rows = ctypes.c_uint64()
+    bad = _lib.MRS_ERR_INVALID_ARGUMENT
+    assert lib.mrs_route_max_rows(None, ctypes.byref(rows)) == bad
+    assert lib.mrs_route_create(None, ctypes.byref(_desc()), None) == bad
+    assert lib.mrs_route_destroy(None) == _lib.MRS_OK
+    assert lib.mrs_route_select(None, 1, None, 8, 0, None, None, None, None) == bad
+    assert lib.mrs_route_select_backward(None, 1, None, 8, 0, None, None, None, None, 8, None) == bad
+    assert lib.mrs_route_order(None, 1, None, None, None) == bad
+    assert lib.mrs_route_dispatch(None, 1, None, 0, 8, None, 8, None, 8, None) == bad
+    assert lib.mrs_route_dispatch_backward(None, 1, None, 0, 8, None, 8, None, 8, None) == bad
+    assert lib.mrs_route_combine(None, 1, None, 0, 8, None, 8, None, None, 8, None) == bad
+    assert lib.mrs_route_combine_backward(None, 1, None, 0, 8, None, 8, None, 8, None, None, 8, None, None) == bad
+
+
+def _plan_on_the_cpu(tokens=4, experts=8, topk=2):
+    """The Python checks alone: a plan without a handle, on CPU tensors."""
+    plan = object.__new__(mrs.RoutePlan)
+    plan.ctx, plan.lib, plan._h = types.SimpleNamespace(device=torch.device("cpu")), _lib.load_library(), None
+    plan.tokens, plan.experts, plan.topk, plan.max_rows = tokens, experts, topk, tokens * topk
+    return plan
+
+
+def test_tensor_checks(monkeypatch):
+    from wgpu_morton_code_radix_sort_test_amd import api
+
+    monkeypatch.setattr(api, "_stream", lambda stream: None)
+    plan = _plan_on_the_cpu()
+    route = plan.new_map()
+    x, rows = torch.zeros(4, 6), torch.zeros(8, 6)
+    ids, w = torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2)
+    scores = torch.zeros(4, 8)
+    # right arguments get as far as the library, which misses the handle
+    for call in (lambda: plan.select(scores), lambda: plan.select_backward(scores, ids, w), lambda: plan.order(ids, route),
+                 lambda: plan.dispatch(x, route), lambda: plan.dispatch_backward(rows, route), lambda: plan.combine(rows, route, w),
+                 lambda: plan.combine_backward(x, rows, route, w), lambda: plan.dispatch(x.to(torch.uint8), route)):
+        with pytest.raises(mrs.MrsError, match="null handle"):
+            call()
+    wrong = [
+        lambda: plan.select(torch.zeros(4, 7)), lambda: plan.select(torch.zeros(4, 8, dtype=torch.float64)),
+        lambda: plan.select(torch.zeros(8, 4).t()), lambda: plan.select(scores, torch.zeros(7)),
+        lambda: plan.select(scores, torch.zeros(8, dtype=torch.float16)), lambda: plan.select(torch.zeros(8)),
+        lambda: plan.select(scores, ids_out=torch.zeros(4, 2, dtype=torch.int64)),
+        lambda: plan.select(scores, weights_out=torch.zeros(3, 2)),
+        lambda: plan.select_backward(scores, ids.long(), w), lambda: plan.select_backward(scores, ids, w.half()),
+        lambda: plan.select_backward(scores, ids, w, scores_grad_out=torch.zeros(4, 8, dtype=torch.float16)),
+        lambda: plan.order(ids.long()), lambda: plan.order(ids[:, :1]), lambda: plan.order(ids.t().contiguous().t(), route),
+        lambda: plan.order(torch.zeros(5, 2, dtype=torch.int32), route),  # more tokens than the map holds
+        lambda: plan.dispatch(x.double(), route), lambda: plan.dispatch(torch.zeros(6, 4).t(), route),
+        lambda: plan.dispatch(x, route, rows_out=torch.zeros(8, 5)), lambda: plan.dispatch(x, route, rows_out=rows.half()),
+        lambda: plan.dispatch(torch.zeros(5, 6), route), lambda: plan.dispatch(torch.zeros(6), route),
+        lambda: plan.dispatch_backward(rows.to(torch.uint8), route), lambda: plan.dispatch_backward(rows[:7], route),
+        lambda: plan.combine(rows, route, w.half()), lambda: plan.combine(rows, route, w, out=torch.zeros(4, 7)),
+        lambda: plan.combine(rows, route, torch.zeros(2)), lambda: plan.combine(rows.t().contiguous().t(), route, w),
+        lambda: plan.combine_backward(x.half(), rows, route, w), lambda: plan.combine_backward(x[:3], rows, route, w),
+        lambda: plan.combine_backward(x, rows, route, w, dweights_out=torch.zeros(4, 2, dtype=torch.float16)),
+        lambda: plan.dispatch(x, mrs.RouteMap(route.row_of_slot.long(), route.slot_of_row, route.counts, route.offsets)),
+        lambda: plan.dispatch(x, mrs.RouteMap(route.row_of_slot, route.slot_of_row, route.counts, route.offsets[:8])),
+    ]
+    for i, call in enumerate(wrong):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+    plan.ctx.device = torch.device("cuda", 0)  # tensors elsewhere than the plan
+    with pytest.raises(ValueError, match="is on"):
+        plan.dispatch(x, route)
+
+
+@pytest.mark.parametrize("gate", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("normalize", [False, True])
+def test_derivative_formula_matches_differences(gate, normalize):
+    """Central differences of the definition in 64 bits: an error of h^2 / 6 times the third derivative, which is
+    below 60 for |dw| <= 1 (cumulants of at most unit variables), and of 2^-52 / h: together below 1e-7 for h = 2^-14."""
+    g = torch.Generator().manual_seed(1)
+    s = (torch.randperm(12, generator=g).double() * 0.25 - 1).reshape(1, 12)
+    s[0, 3] = -ref.INF
+    ids = ref.select_ids(s, None, 4)
+    dw = torch.rand(1, 4, generator=g, dtype=torch.float64) * 2 - 1
+    got = ref.scores_grad(s, None, ids, dw, gate, normalize, 1.5)
+    h = 2.0**-14
+    for e in range(12):
+        up, down = s.clone(), s.clone()
+        up[0, e] += h
+        down[0, e] -= h
+        f = [float((ref.weights(x, None, ids, gate, normalize, 1.5) * dw).sum()) for x in (up, down)]
+        want = 0.0 if e == 3 else (f[0] - f[1]) / (2 * h)
+        assert abs(float(got[0, e]) - want) < 1e-7 * 1.5

@@ -10,7 +10,11 @@ from .api import (  # noqa: F401
     ALGO_ONESWEEP,
     ALGO_THREE_KERNEL,
     Context,
+    GATE_SIGMOID,
+    GATE_SOFTMAX,
     PlanInfo,
+    RouteMap,
+    RoutePlan,
     SortPlan,
 )
 from . import scene  # noqa: F401

@@ -90,11 +90,35 @@ class DistInfoStruct(ctypes.Structure):
     ]
 
 
+class RouteDesc(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_uint64),
+        ("experts", ctypes.c_int32),
+        ("topk", ctypes.c_int32),
+        ("align", ctypes.c_int32),
+        ("gate", ctypes.c_int32),
+        ("capacity", ctypes.c_uint64),
+        ("normalize", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class RouteMapStruct(ctypes.Structure):
+    _fields_ = [
+        ("row_of_slot", ctypes.c_void_p),
+        ("slot_of_row", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("rows", ctypes.c_uint64),
+    ]
+
+
 _vp = ctypes.c_void_p
 _u64 = ctypes.c_uint64
 _u32 = ctypes.c_uint32
 _i32 = ctypes.c_int32
 _fp = ctypes.POINTER(ctypes.c_float)
+_map = ctypes.POINTER(RouteMapStruct)
 
 # name -> (restype, argtypes); every symbol include/mrs.h declares
 SIGNATURES = {
@@ -146,6 +170,16 @@ SIGNATURES = {
     "mrs_splitter_next": (ctypes.c_int, [_vp, ctypes.POINTER(_u32), ctypes.POINTER(_u32), ctypes.POINTER(_u32), ctypes.POINTER(_u64)]),
     "mrs_splitter_feed": (ctypes.c_int, [_vp, _vp]),
     "mrs_splitter_get": (ctypes.c_int, [_vp, _vp]),
+    "mrs_route_create": (ctypes.c_int, [_vp, ctypes.POINTER(RouteDesc), ctypes.POINTER(_vp)]),
+    "mrs_route_destroy": (ctypes.c_int, [_vp]),
+    "mrs_route_max_rows": (ctypes.c_int, [ctypes.POINTER(RouteDesc), ctypes.POINTER(_u64)]),
+    "mrs_route_select": (ctypes.c_int, [_vp, _u64, _vp, _u64, _i32, _vp, _vp, _vp, _vp]),
+    "mrs_route_select_backward": (ctypes.c_int, [_vp, _u64, _vp, _u64, _i32, _vp, _vp, _vp, _vp, _u64, _vp]),
+    "mrs_route_order": (ctypes.c_int, [_vp, _u64, _vp, _map, _vp]),
+    "mrs_route_dispatch": (ctypes.c_int, [_vp, _u64, _map, _i32, _u64, _vp, _u64, _vp, _u64, _vp]),
+    "mrs_route_dispatch_backward": (ctypes.c_int, [_vp, _u64, _map, _i32, _u64, _vp, _u64, _vp, _u64, _vp]),
+    "mrs_route_combine": (ctypes.c_int, [_vp, _u64, _map, _i32, _u64, _vp, _u64, _vp, _vp, _u64, _vp]),
+    "mrs_route_combine_backward": (ctypes.c_int, [_vp, _u64, _map, _i32, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _u64, _vp, _vp]),
     "mrs_generate_points": (ctypes.c_int, [_vp, _u64, _u64, _vp, _vp]),
     "mrs_generate_u32": (ctypes.c_int, [_vp, _u64, _u64, _u64, _vp, _vp]),
 }

@@ -16,6 +16,9 @@ ALGO_THREE_KERNEL = 0
 ALGO_ONESWEEP = 1
 ALGO_HYBRID = 2
 
+GATE_SOFTMAX = 0
+GATE_SIGMOID = 1
+
 MORTON_UNIFORMS_BYTES = 51248
 VERTEX_STRIDE = 48
 TRIANGLE_STRIDE = 16
@@ -399,3 +402,235 @@ class SortPlan:
         buckets, groups = ctypes.c_uint32(0), ctypes.c_uint32(0)
         _lib.check(self.lib.mrs_plan_get_adaptive(self._h, _stream(stream), ctypes.byref(buckets), ctypes.byref(groups)))
         return buckets.value, groups.value
+
+
+# MRS_TYPE_* of the element types rows can have
+_ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_TYPE_8BIT = 3
+
+
+@dataclass(frozen=True)
+class RouteMap:
+    """`mrs_route_map`: int32 device tensors that say where every slot's row is.  `row_of_slot` [tokens,
+    topk] holds a row or -1, `slot_of_row` [rows] a slot (token * topk + j) or -1, `counts` [experts] the rows an
+    expert has, `offsets` [experts + 1] where its segment starts and, last, where all of them end."""
+
+    row_of_slot: torch.Tensor
+    slot_of_row: torch.Tensor
+    counts: torch.Tensor
+    offsets: torch.Tensor
+
+
+class RoutePlan:
+    """`mrs_route`: tokens routed to experts.  Every one of at most `tokens` tokens has `topk` slots; `select`
+    picks their experts, `order` sorts the slots by expert, `dispatch` moves the tokens' rows into that
+    order, `combine` brings them back weighted; the `*_backward` calls are the gradients.  An expert's rows start
+    at a multiple of `align`; beyond `capacity` rows (0 = no limit) its later slots are dropped.  `gate`,
+    `normalize` and `scale` say how scores become weights (include/mrs.h).  One handle runs one `order` at a time."""
+
+    def __init__(self, ctx, tokens, experts, topk, align=1, capacity=0, gate=GATE_SOFTMAX, normalize=True, scale=1.0):
+        self._h = None
+        self.ctx = ctx
+        self.lib = ctx.lib
+        for name, v in (("tokens", tokens), ("capacity", capacity)):
+            if v < 0:
+                raise ValueError(f"{name} must not be negative")
+        self.desc = _lib.RouteDesc(tokens, experts, topk, align, gate, capacity, 1 if normalize else 0, scale)
+        rows = ctypes.c_uint64()
+        _lib.check(self.lib.mrs_route_max_rows(ctypes.byref(self.desc), ctypes.byref(rows)))
+        handle = ctypes.c_void_p()
+        _lib.check(self.lib.mrs_route_create(ctx._h, ctypes.byref(self.desc), ctypes.byref(handle)))
+        self._h = handle
+        self.tokens, self.experts, self.topk = tokens, experts, topk
+        self.max_rows = rows.value
+
+    def close(self):
+        if self._h:
+            self.lib.mrs_route_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    # ---- checks --------------------------------------------------------------------
+    def _on_device(self, t, name):
+        if t.device != self.ctx.device:
+            raise ValueError(f"{name} is on {t.device}, the plan on {self.ctx.device}")
+
+    def _rows(self, t, name, rows, hidden, dtype):
+        """Pointer and row stride of a matrix whose rows are contiguous."""
+        self._on_device(t, name)
+        if t.dim() != 2 or t.size(0) != rows or t.size(1) != hidden:
+            raise ValueError(f"{name} must have shape [{rows}, {hidden}], not {list(t.shape)}")
+        if t.dtype != dtype:
+            raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+        ld = t.stride(0)
+        if hidden > 1 and t.stride(1) != 1:
+            raise ValueError(f"the rows of {name} must be contiguous")
+        if rows <= 1 and ld < hidden:
+            ld = hidden
+        return t.data_ptr(), ld
+
+    def _per_slot(self, t, name, tokens, dtype):
+        self._on_device(t, name)
+        if t.dtype != dtype or t.dim() != 2 or t.size(0) != tokens or t.size(1) != self.topk or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape [{tokens}, {self.topk}]")
+        return t.data_ptr()
+
+    def _slots(self, t, name):
+        if t.dim() != 2:
+            raise ValueError(f"{name} must have two dimensions, not {t.dim()}")
+        return t.size(0)
+
+    def _map(self, route, tokens):
+        rows = route.slot_of_row.numel()
+        for t, name, least in ((route.row_of_slot, "row_of_slot", tokens * self.topk), (route.slot_of_row, "slot_of_row", 0),
+                               (route.counts, "counts", self.experts), (route.offsets, "offsets", self.experts + 1)):
+            self._on_device(t, name)
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < least:
+                raise ValueError(f"{name} must be a contiguous int32 tensor of at least {least} elements")
+        return ctypes.byref(_lib.RouteMapStruct(route.row_of_slot.data_ptr(), route.slot_of_row.data_ptr(),
+                                                route.counts.data_ptr(), route.offsets.data_ptr(), rows)), rows
+
+    def _row_type(self, t, name, eight_bits=False):
+        if t.dim() != 2:
+            raise ValueError(f"{name} must have two dimensions, not {t.dim()}")
+        kind = _ROW_TYPES.get(t.dtype)
+        if kind is None and eight_bits and t.element_size() == 1:
+            kind = _TYPE_8BIT
+        if kind is None:
+            raise ValueError(f"{name} has the unsupported type {t.dtype}")
+        return kind
+
+    def _bias(self, bias):
+        if bias is None:
+            return None
+        self._on_device(bias, "bias")
+        if bias.dtype != torch.float32 or bias.numel() != self.experts or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous float32 tensor of {self.experts} elements")
+        return bias.data_ptr()
+
+    def _scores(self, scores):
+        kind = self._row_type(scores, "scores")
+        tokens = scores.size(0)
+        ptr, ld = self._rows(scores, "scores", tokens, self.experts, scores.dtype)
+        return tokens, kind, ptr, ld
+
+    # ---- calls -----------------------------------------------------------------------
+    def new_map(self, tokens=None):
+        """An unwritten RouteMap for `order` calls of `tokens` tokens (the plan's, by default)."""
+        tokens = self.tokens if tokens is None else tokens
+        make = lambda *shape: torch.empty(shape, dtype=torch.int32, device=self.ctx.device)  # noqa: E731
+        return RouteMap(make(tokens, self.topk), make(self.max_rows), make(self.experts), make(self.experts + 1))
+
+    def select(self, scores, bias=None, ids_out=None, weights_out=None, stream=None):
+        """`mrs_route_select`: the topk experts of every token and their weights, (ids int32, weights float32), both
+        [tokens, topk], from scores [tokens, experts] (float32, float16 or bfloat16)."""
+        tokens, kind, ptr, ld = self._scores(scores)
+        if ids_out is None:
+            ids_out = torch.empty((tokens, self.topk), dtype=torch.int32, device=self.ctx.device)
+        if weights_out is None:
+            weights_out = torch.empty((tokens, self.topk), dtype=torch.float32, device=self.ctx.device)
+        _lib.check(
+            self.lib.mrs_route_select(self._h, tokens, ptr, ld, kind, self._bias(bias),
+                                      self._per_slot(ids_out, "ids_out", tokens, torch.int32),
+                                      self._per_slot(weights_out, "weights_out", tokens, torch.float32), _stream(stream))
+        )
+        return ids_out, weights_out
+
+    def select_backward(self, scores, ids, weights_grad, bias=None, scores_grad_out=None, stream=None):
+        """`mrs_route_select_backward`: the gradient of `scores`, of their type, from that of the weights."""
+        tokens, kind, ptr, ld = self._scores(scores)
+        if scores_grad_out is None:
+            scores_grad_out = torch.empty((tokens, self.experts), dtype=scores.dtype, device=self.ctx.device)
+        grad_ptr, grad_ld = self._rows(scores_grad_out, "scores_grad_out", tokens, self.experts, scores.dtype)
+        _lib.check(
+            self.lib.mrs_route_select_backward(self._h, tokens, ptr, ld, kind, self._bias(bias),
+                                               self._per_slot(ids, "ids", tokens, torch.int32),
+                                               self._per_slot(weights_grad, "weights_grad", tokens, torch.float32),
+                                               grad_ptr, grad_ld, _stream(stream))
+        )
+        return scores_grad_out
+
+    def order(self, ids, map_out=None, stream=None):
+        """`mrs_route_order`: a RouteMap of the slots sorted by ids [tokens, topk] (int32; ids outside [0, experts)
+        get no row).  Every tensor of `map_out` is written."""
+        tokens = self._slots(ids, "ids")
+        ids_ptr = self._per_slot(ids, "ids", tokens, torch.int32)
+        if map_out is None:
+            map_out = self.new_map(tokens)
+        raw, _ = self._map(map_out, tokens)
+        _lib.check(self.lib.mrs_route_order(self._h, tokens, ids_ptr, raw, _stream(stream)))
+        return map_out
+
+    def dispatch(self, x, route, rows_out=None, stream=None):
+        """`mrs_route_dispatch`: x [tokens, hidden] in expert order, [rows, hidden].  Rows behind the last segment are
+        left as they are: in an own `rows_out` that is what was there, in a new tensor anything."""
+        kind = self._row_type(x, "x", eight_bits=True)
+        tokens, hidden = x.size(0), x.size(1)
+        raw, rows = self._map(route, tokens)
+        x_ptr, ld_x = self._rows(x, "x", tokens, hidden, x.dtype)
+        if rows_out is None:
+            rows_out = torch.empty((rows, hidden), dtype=x.dtype, device=self.ctx.device)
+        out_ptr, ld_out = self._rows(rows_out, "rows_out", rows, hidden, x.dtype)
+        _lib.check(self.lib.mrs_route_dispatch(self._h, tokens, raw, kind, hidden, x_ptr, ld_x, out_ptr, ld_out, _stream(stream)))
+        return rows_out
+
+    def dispatch_backward(self, rows_grad, route, x_grad_out=None, tokens=None, stream=None):
+        """`mrs_route_dispatch_backward`: the gradient of x [tokens, hidden]; `tokens` by default those of the map."""
+        kind = self._row_type(rows_grad, "rows_grad")
+        hidden = rows_grad.size(1)
+        tokens = self._tokens_of(route, tokens)
+        raw, rows = self._map(route, tokens)
+        in_ptr, ld_in = self._rows(rows_grad, "rows_grad", rows, hidden, rows_grad.dtype)
+        if x_grad_out is None:
+            x_grad_out = torch.empty((tokens, hidden), dtype=rows_grad.dtype, device=self.ctx.device)
+        out_ptr, ld_out = self._rows(x_grad_out, "x_grad_out", tokens, hidden, rows_grad.dtype)
+        _lib.check(
+            self.lib.mrs_route_dispatch_backward(self._h, tokens, raw, kind, hidden, in_ptr, ld_in, out_ptr, ld_out,
+                                                 _stream(stream))
+        )
+        return x_grad_out
+
+    def combine(self, rows, route, weights, out=None, stream=None):
+        """`mrs_route_combine`: out[t] = sum over j of weights[t, j] * rows[row_of_slot[t, j]], of the rows' type."""
+        kind = self._row_type(rows, "rows")
+        tokens, hidden = self._slots(weights, "weights"), rows.size(1)
+        raw, count = self._map(route, tokens)
+        in_ptr, ld_in = self._rows(rows, "rows", count, hidden, rows.dtype)
+        if out is None:
+            out = torch.empty((tokens, hidden), dtype=rows.dtype, device=self.ctx.device)
+        out_ptr, ld_out = self._rows(out, "out", tokens, hidden, rows.dtype)
+        _lib.check(
+            self.lib.mrs_route_combine(self._h, tokens, raw, kind, hidden, in_ptr, ld_in,
+                                       self._per_slot(weights, "weights", tokens, torch.float32), out_ptr, ld_out,
+                                       _stream(stream))
+        )
+        return out
+
+    def combine_backward(self, out_grad, rows, route, weights, drows_out=None, dweights_out=None, stream=None):
+        """`mrs_route_combine_backward`: (gradient of rows, gradient of weights float32).  Rows behind the last segment
+        are left as they are, as in `dispatch`."""
+        kind = self._row_type(rows, "rows")
+        tokens, hidden = self._slots(weights, "weights"), rows.size(1)
+        raw, count = self._map(route, tokens)
+        grad_ptr, ld_grad = self._rows(out_grad, "out_grad", tokens, hidden, rows.dtype)
+        in_ptr, ld_in = self._rows(rows, "rows", count, hidden, rows.dtype)
+        if drows_out is None:
+            drows_out = torch.empty((count, hidden), dtype=rows.dtype, device=self.ctx.device)
+        if dweights_out is None:
+            dweights_out = torch.empty((tokens, self.topk), dtype=torch.float32, device=self.ctx.device)
+        out_ptr, ld_out = self._rows(drows_out, "drows_out", count, hidden, rows.dtype)
+        _lib.check(
+            self.lib.mrs_route_combine_backward(self._h, tokens, raw, kind, hidden, grad_ptr, ld_grad, in_ptr, ld_in,
+                                                self._per_slot(weights, "weights", tokens, torch.float32), out_ptr, ld_out,
+                                                self._per_slot(dweights_out, "dweights_out", tokens, torch.float32),
+                                                _stream(stream))
+        )
+        return drows_out, dweights_out
+
+    def _tokens_of(self, route, tokens):
+        return route.row_of_slot.numel() // self.topk if tokens is None else tokens

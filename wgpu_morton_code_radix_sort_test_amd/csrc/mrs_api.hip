@@ -233,7 +233,7 @@ static bool stream_is_capturing(hipStream_t s)
     return st != hipStreamCaptureStatusNone;
 }
 
-static int check_device(const mrs_context* ctx, const char* who)
+int check_device(const mrs_context* ctx, const char* who)
 {
     int cur = -1;
     MRS_HIP_TRY(hipGetDevice(&cur));

@@ -19,6 +19,8 @@ int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 void clear_error();
 // Zeroes `bytes` of device memory (address and size multiples of 4) behind the work already on `s`.
 int clear_async(void* p, size_t bytes, hipStream_t s);
+// MRS_ERR_INVALID_ARGUMENT unless the calling thread's current device is the context's (mrs_api.hip).
+int check_device(const mrs_context* ctx, const char* who);
 
 #define MRS_HIP_TRY(expr)                                                              \
     do {                                                                               \

@@ -1,0 +1,297 @@
+// Stable counting sort of token slots by expert (mrs_route_order in include/mrs.h).
+//
+// row(slot) = offset of its expert + how many earlier kept slots have the same expert.  A workgroup
+// ranks `16 waves x 64 lanes x R` consecutive slots at a time: a wave takes 64 neighbouring slots, finds
+// the lanes with the same expert by one ballot per bit of its number, and adds their count to its own
+// counter of that expert, so that a slot's rank inside the wave's stretch is the counter before plus
+// the equal lanes below; a scan over the waves' counters gives the rank inside the tile.  No
+// atomics decide an order, so rows are the same every time.
+//
+// Up to kSmallSlots slots one workgroup does everything in one launch; what bounds it is the chain of
+// LDS accesses and barriers.  Above, a first launch counts tiles, and in a second one
+// every workgroup adds up the counts of the tiles before its own by itself (at most 256 tiles of
+// `experts` counts, read from L2) instead of waiting for a scan launch between the two.
+#include "mrs_route.hpp"
+
+namespace mrs {
+
+namespace {
+
+constexpr uint32_t kWaves = 16;
+constexpr uint32_t kThreads = kWaves * 64;
+constexpr uint32_t kMaxExperts = MRS_ROUTE_MAX_EXPERTS;
+static_assert(kMaxExperts <= kThreads, "one thread per expert in the scans");
+constexpr uint32_t kSmallR = 8;
+constexpr uint32_t kSmallSlots = kThreads * kSmallR;
+constexpr uint32_t kTileR = 4;
+constexpr uint32_t kTileSlots = kThreads * kTileR;
+
+struct OrderShared {
+    uint16_t wave_count[kWaves][kMaxExperts];  // slots per wave, then those of the waves before
+    uint32_t row[kMaxExperts];                 // first row of the expert in this tile
+    uint32_t room[kMaxExperts];                // rows it may still take
+    uint32_t wave_sum[kWaves];
+};
+
+// Lanes of the wave that hold the same value; `bits` significant bits.
+__device__ __forceinline__ uint64_t same_value(uint32_t v, uint32_t bits)
+{
+    uint64_t same = ~0ull;
+    for (uint32_t b = 0; b < bits; ++b) {
+        const bool set = (v >> b) & 1u;
+        const uint64_t with = __ballot(set);
+        same &= set ? with : ~with;
+    }
+    return same;
+}
+
+// Exclusive scan of one value per thread over the workgroup; *total is the sum of all.
+__device__ __forceinline__ uint32_t block_exclusive_scan(uint32_t v, uint32_t* wave_sum, uint32_t* total)
+{
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t incl = v;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint32_t up = __shfl_up(incl, d);
+        if (lane >= d) incl += up;
+    }
+    if (lane == 63) wave_sum[wave] = incl;
+    __syncthreads();
+    uint32_t before = 0, sum = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) {
+        const uint32_t x = wave_sum[w];
+        if (w < wave) before += x;
+        sum += x;
+    }
+    *total = sum;
+    return before + incl - v;
+}
+
+__device__ __forceinline__ uint32_t round_up_to(uint32_t v, uint32_t a) { return (v + a - 1) / a * a; }
+
+// Loads a tile's experts (`experts` where a slot has none) and ranks them inside their waves; the
+// waves' counters must be zero.
+template <uint32_t R>
+__device__ __forceinline__ void rank_in_waves(const OrderArgs& a, OrderShared& sh, uint64_t first, uint32_t bits,
+                                              uint32_t (&expert)[R], uint32_t (&rank)[R])
+{
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint64_t mine = first + wave * (64u * R) + lane;
+#pragma unroll
+    for (uint32_t i = 0; i < R; ++i) {
+        const uint64_t slot = mine + i * 64u;
+        expert[i] = slot < a.slots ? static_cast<uint32_t>(a.ids[slot]) : a.experts;
+    }
+    volatile uint16_t* count = sh.wave_count[wave];
+#pragma unroll
+    for (uint32_t i = 0; i < R; ++i) {
+        if (expert[i] > a.experts) expert[i] = a.experts;
+        const uint64_t same = same_value(expert[i], bits);
+        const uint32_t below = __popcll(same & ((1ull << lane) - 1ull));
+        rank[i] = below;
+        if (expert[i] < a.experts) {
+            const uint32_t before = count[expert[i]];
+            rank[i] += before;
+            if (below == 0) count[expert[i]] = static_cast<uint16_t>(before + __popcll(same));
+        }
+    }
+}
+
+// Turns thread e's column of counters into those of the waves before; returns the tile's sum.
+__device__ __forceinline__ uint32_t scan_waves(OrderShared& sh, uint32_t e)
+{
+    uint32_t c[kWaves];
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) c[w] = sh.wave_count[w][e];
+    uint32_t run = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) {
+        sh.wave_count[w][e] = static_cast<uint16_t>(run);
+        run += c[w];
+    }
+    return run;
+}
+
+template <uint32_t R>
+__device__ __forceinline__ void write_rows(const OrderArgs& a, const OrderShared& sh, uint64_t first,
+                                           const uint32_t (&expert)[R], const uint32_t (&rank)[R])
+{
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint64_t mine = first + wave * (64u * R) + lane;
+#pragma unroll
+    for (uint32_t i = 0; i < R; ++i) {
+        const uint64_t slot = mine + i * 64u;
+        if (slot >= a.slots) continue;
+        int32_t row = -1;
+        if (expert[i] < a.experts) {
+            const uint32_t in_tile = sh.wave_count[wave][expert[i]] + rank[i];
+            if (in_tile < sh.room[expert[i]]) {
+                row = static_cast<int32_t>(sh.row[expert[i]] + in_tile);
+                if (static_cast<uint32_t>(row) < a.rows) a.slot_of_row[row] = static_cast<int32_t>(slot);
+            }
+        }
+        a.row_of_slot[slot] = row;
+    }
+}
+
+// Rows without a slot: what fills the segments up, and everything behind the last one.
+__device__ __forceinline__ void mark_empty_rows(const OrderArgs& a, uint32_t e, uint32_t begin, uint32_t end)
+{
+    (void)e;
+    if (end > a.rows) end = a.rows;
+    for (uint32_t r = begin; r < end; ++r) a.slot_of_row[r] = -1;
+}
+
+__global__ __launch_bounds__(kThreads) void route_order_small_kernel(const OrderArgs a, uint32_t bits)
+{
+    __shared__ OrderShared sh;
+    const uint32_t tid = threadIdx.x;
+    for (uint32_t i = tid; i < kWaves * a.experts; i += kThreads) sh.wave_count[i / a.experts][i % a.experts] = 0;
+    __syncthreads();
+    uint32_t expert[kSmallR], rank[kSmallR];
+    rank_in_waves<kSmallR>(a, sh, 0, bits, expert, rank);
+    __syncthreads();
+    uint32_t kept = 0;
+    if (tid < a.experts) {
+        kept = scan_waves(sh, tid);
+        if (kept > a.capacity) kept = a.capacity;
+    }
+    const uint32_t padded = round_up_to(kept, a.align);
+    uint32_t end;
+    const uint32_t offset = block_exclusive_scan(padded, sh.wave_sum, &end);
+    if (tid < a.experts) {
+        sh.row[tid] = offset;
+        sh.room[tid] = a.capacity;
+        a.counts[tid] = static_cast<int32_t>(kept);
+        a.offsets[tid] = static_cast<int32_t>(offset);
+        if (tid == a.experts - 1) a.offsets[a.experts] = static_cast<int32_t>(end);
+        mark_empty_rows(a, tid, offset + kept, offset + padded);
+    }
+    for (uint64_t r = static_cast<uint64_t>(end) + tid; r < a.rows; r += kThreads) a.slot_of_row[r] = -1;
+    __syncthreads();
+    write_rows<kSmallR>(a, sh, 0, expert, rank);
+}
+
+// tile_counts[block][e] = slots of expert e in the block's stretch of `per_block` slots
+__global__ __launch_bounds__(kThreads) void route_order_count_kernel(const OrderArgs a, uint64_t per_block, uint32_t stride)
+{
+    __shared__ uint32_t count[kMaxExperts];
+    const uint32_t tid = threadIdx.x;
+    if (tid < a.experts) count[tid] = 0;
+    __syncthreads();
+    const uint64_t first = blockIdx.x * per_block;
+    uint64_t last = first + per_block;
+    if (last > a.slots) last = a.slots;
+    for (uint64_t slot = first + tid; slot < last; slot += kThreads) {
+        const uint32_t e = static_cast<uint32_t>(a.ids[slot]);
+        if (e < a.experts) atomicAdd(&count[e], 1u);
+    }
+    __syncthreads();
+    if (tid < a.experts) a.tile_counts[static_cast<uint64_t>(blockIdx.x) * stride + tid] = count[tid];
+}
+
+__global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a, uint64_t per_block, uint32_t stride, uint32_t bits)
+{
+    __shared__ OrderShared sh;
+    __shared__ uint32_t before_me[kMaxExperts];
+    __shared__ uint32_t of_all[kMaxExperts];
+    const uint32_t tid = threadIdx.x;
+    if (tid < a.experts) {
+        before_me[tid] = 0;
+        of_all[tid] = 0;
+    }
+    __syncthreads();
+    // the counts of all tiles, four experts a thread, the tiles shared out among groups of threads
+    const uint32_t quads = stride / 4;
+    const uint32_t groups = kThreads / quads;
+    const uint32_t group = tid / quads;
+    if (group < groups) {
+        const uint32_t e = (tid - group * quads) * 4;
+        uint32_t before[4] = {0, 0, 0, 0}, all[4] = {0, 0, 0, 0};
+#pragma unroll 8
+        for (uint32_t t = group; t < gridDim.x; t += groups) {
+            const uint4 c = *reinterpret_cast<const uint4*>(a.tile_counts + static_cast<uint64_t>(t) * stride + e);
+            const uint32_t mask = t < blockIdx.x ? 0xFFFFFFFFu : 0u;
+            all[0] += c.x, all[1] += c.y, all[2] += c.z, all[3] += c.w;
+            before[0] += c.x & mask, before[1] += c.y & mask, before[2] += c.z & mask, before[3] += c.w & mask;
+        }
+        // whole numbers: the order of these additions does not matter
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (e + i < a.experts) {
+                atomicAdd(&of_all[e + i], all[i]);
+                atomicAdd(&before_me[e + i], before[i]);
+            }
+    }
+    __syncthreads();
+    uint32_t kept = 0, taken = 0;
+    if (tid < a.experts) {
+        kept = of_all[tid];
+        if (kept > a.capacity) kept = a.capacity;
+        taken = before_me[tid];
+        if (taken > a.capacity) taken = a.capacity;
+    }
+    const uint32_t padded = round_up_to(kept, a.align);
+    uint32_t end;
+    const uint32_t offset = block_exclusive_scan(padded, sh.wave_sum, &end);
+    if (tid < a.experts) {
+        sh.row[tid] = offset + taken;
+        sh.room[tid] = a.capacity - taken;
+        if (blockIdx.x == 0) {
+            a.counts[tid] = static_cast<int32_t>(kept);
+            a.offsets[tid] = static_cast<int32_t>(offset);
+            if (tid == a.experts - 1) a.offsets[a.experts] = static_cast<int32_t>(end);
+        }
+        if (tid % gridDim.x == blockIdx.x) mark_empty_rows(a, tid, offset + kept, offset + padded);
+    }
+    for (uint64_t r = static_cast<uint64_t>(end) + static_cast<uint64_t>(blockIdx.x) * kThreads + tid; r < a.rows;
+         r += static_cast<uint64_t>(gridDim.x) * kThreads)
+        a.slot_of_row[r] = -1;
+
+    const uint64_t first = blockIdx.x * per_block;
+    uint64_t last = first + per_block;
+    if (last > a.slots) last = a.slots;
+    for (uint64_t at = first; at < last; at += kTileSlots) {
+        for (uint32_t i = tid; i < kWaves * a.experts; i += kThreads) sh.wave_count[i / a.experts][i % a.experts] = 0;
+        __syncthreads();
+        uint32_t expert[kTileR], rank[kTileR];
+        rank_in_waves<kTileR>(a, sh, at, bits, expert, rank);
+        __syncthreads();
+        uint32_t in_tile = 0;
+        if (tid < a.experts) in_tile = scan_waves(sh, tid);
+        __syncthreads();
+        write_rows<kTileR>(a, sh, at, expert, rank);
+        __syncthreads();
+        if (tid < a.experts) {
+            const uint32_t room = sh.room[tid];
+            const uint32_t took = in_tile < room ? in_tile : room;
+            sh.row[tid] += took;
+            sh.room[tid] = room - took;
+        }
+    }
+}
+
+}  // namespace
+
+int launch_route_order(const OrderArgs& a, hipStream_t s)
+{
+    uint32_t bits = 0;
+    while ((a.experts >> bits) != 0) ++bits;  // the values 0 .. experts
+    if (a.slots <= kSmallSlots) {
+        hipLaunchKernelGGL(route_order_small_kernel, dim3(1), dim3(kThreads), 0, s, a, bits);
+        MRS_CHECK_LAUNCH("route_order_small_kernel");
+        return MRS_OK;
+    }
+    const uint32_t stride = (a.experts + 3) / 4 * 4;
+    uint64_t tiles = (a.slots + kTileSlots - 1) / kTileSlots;
+    const uint64_t per_block = (tiles + kRouteMaxTiles - 1) / kRouteMaxTiles * kTileSlots;
+    const uint32_t blocks = static_cast<uint32_t>((a.slots + per_block - 1) / per_block);
+    hipLaunchKernelGGL(route_order_count_kernel, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride);
+    MRS_CHECK_LAUNCH("route_order_count_kernel");
+    hipLaunchKernelGGL(route_order_kernel, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride, bits);
+    MRS_CHECK_LAUNCH("route_order_kernel");
+    return MRS_OK;
+}
+
+}  // namespace mrs
