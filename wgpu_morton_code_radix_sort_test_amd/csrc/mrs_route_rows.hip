@@ -6,48 +6,76 @@
 
 #include "mrs_route.hpp"
 
+
 namespace mrs {
 
 namespace {
 
-constexpr uint32_t kThreads = 256;
-constexpr uint64_t kMaxBlocks = 1u << 22;  // more work than that is looped over
+constexpr uint32_t kMoveThreads = 128;   // dispatch
+constexpr uint32_t kSumThreads = 1024;   // combine and its gradient: a workgroup covers whole rows
+constexpr uint32_t kMaxBlocks = 1u << 20;  // more work than that is looped over
+// Rows that cannot stay in the 256 MiB memory-side cache until somebody reads them again are streamed past the caches.
+constexpr uint64_t kStreamBytes = 256ull << 20;
 
-// How a launch cuts its work: a token's row in pieces of `lanes` 16-byte vectors (a power of two up
-// to a wave's 64), one item per (token, piece), 256 / lanes items per workgroup.
+// How a launch cuts its work.  A group of `lanes` lanes -- a power of two up to a wave's 64, enough for the row if they can be --
+// takes a piece of a row, a 16-byte vector a lane.
 struct Cut {
     uint32_t lanes_log2;
-    uint32_t vectors;  // vectors of a row, the last one possibly cut short
-    uint32_t pieces;   // ceil(vectors / lanes)
-    uint64_t items;
+    uint32_t vectors;     // whole 16-byte vectors of a row
+    uint32_t pieces;      // of a row
+    uint32_t items;       // what groups take: tokens * pieces, or tokens * token_waves
+    uint32_t token_waves; // combine's gradient: waves that share a token's pieces evenly, a power of two
     uint32_t blocks;      // workgroups for the items
-    uint32_t pad_blocks;  // workgroups behind them that zero the rows between segments' ends
+    uint32_t pad_blocks;  // workgroups before them that zero the rows between segments' ends
     uint32_t pad_split;   // of these, how many share an expert
 };
 
-Cut cut_rows(const MoveArgs& a, uint32_t element_bytes, bool one_item_per_token, bool pads)
+int cut_rows(const MoveArgs& a, uint32_t element_bytes, uint32_t threads, bool whole_tokens, bool pads, Cut* out)
 {
     Cut c;
-    c.vectors = static_cast<uint32_t>((static_cast<uint64_t>(a.hidden) * element_bytes + 15) / 16);
+    const uint64_t row_bytes = static_cast<uint64_t>(a.hidden) * element_bytes;
+    c.vectors = static_cast<uint32_t>(row_bytes / 16);
+    const uint32_t touched = static_cast<uint32_t>((row_bytes + 15) / 16);
     c.lanes_log2 = 0;
-    while (c.lanes_log2 < 6 && (1u << c.lanes_log2) < c.vectors) ++c.lanes_log2;
-    c.pieces = one_item_per_token ? 1 : (c.vectors + (1u << c.lanes_log2) - 1) >> c.lanes_log2;
-    c.items = a.tokens * c.pieces;
-    const uint64_t per_block = kThreads >> c.lanes_log2;
-    uint64_t blocks = (c.items + per_block - 1) / per_block;
+    while (c.lanes_log2 < 6 && (1u << c.lanes_log2) < touched) ++c.lanes_log2;
+    c.pieces = (touched + (1u << c.lanes_log2) - 1) >> c.lanes_log2;
+    c.token_waves = 1;
+    while (c.pieces % (c.token_waves * 2) == 0 && c.token_waves < threads / 64) c.token_waves *= 2;
+    const uint64_t items = a.tokens * (whole_tokens ? c.token_waves : c.pieces);
+    const uint32_t per_block = threads >> c.lanes_log2;
+    uint64_t blocks = (items + per_block - 1) / per_block;
     if (blocks > kMaxBlocks) blocks = kMaxBlocks;
     c.blocks = static_cast<uint32_t>(blocks);
+    // item numbers, and one step beyond the last, fit 32 bits
+    if (items + blocks * per_block > 0xFFFFFFFFull) return fail(MRS_ERR_UNSUPPORTED, "more than 2^32 pieces of rows in one call");
+    c.items = static_cast<uint32_t>(items);
     c.pad_split = 0;
     c.pad_blocks = 0;
     if (pads && a.align > 1) {
         c.pad_split = a.align - 1 < 8 ? a.align - 1 : 8;
         c.pad_blocks = a.experts * c.pad_split;
     }
-    return c;
+    *out = c;
+    return MRS_OK;
+}
+
+template <bool STREAM>
+__device__ __forceinline__ RouteVec get(const void* p)
+{
+    if (STREAM) return __builtin_nontemporal_load(static_cast<const RouteVecLoose*>(p));
+    return load_vec(p);
+}
+template <bool STREAM>
+__device__ __forceinline__ void put(void* p, RouteVec v)
+{
+    if (STREAM)
+        __builtin_nontemporal_store(v, static_cast<RouteVecLoose*>(p));
+    else
+        store_vec(p, v);
 }
 
 // Zeroes the rows of one expert's segment that no slot has.
-template <typename Elem>
+template <typename Elem, uint32_t THREADS>
 __device__ void zero_padding(const MoveArgs& a, const Cut& c, uint32_t block)
 {
     const uint32_t e = block / c.pad_split;
@@ -62,305 +90,371 @@ __device__ void zero_padding(const MoveArgs& a, const Cut& c, uint32_t block)
     const RouteVec zero = {0, 0, 0, 0};
     for (int64_t r = first + part; r < end; r += c.pad_split) {
         Elem* row = out + static_cast<uint64_t>(r) * a.ld_rows_out;
-        for (uint32_t v = threadIdx.x; v < whole; v += kThreads) store_vec(row + static_cast<uint64_t>(v) * N, zero);
-        for (uint32_t h = whole * N + threadIdx.x; h < a.hidden; h += kThreads) row[h] = Elem(0);
+        for (uint32_t v = threadIdx.x; v < whole; v += THREADS) store_vec(row + static_cast<uint64_t>(v) * N, zero);
+        for (uint32_t h = whole * N + threadIdx.x; h < a.hidden; h += THREADS) row[h] = Elem(0);
     }
 }
 
-// The item of this thread: token, piece.  With whole waves on one item the token is the same for all
-// lanes and said to be (its slots' row numbers then come through scalar loads).
-template <bool WAVE>
-__device__ __forceinline__ uint64_t first_item(const Cut& c)
+// This group's first item.  Whole waves on one item say so: what depends on the token alone then lives in
+// scalar registers and comes through scalar loads.
+template <uint32_t THREADS, bool WAVE>
+__device__ __forceinline__ uint32_t first_item(const Cut& c)
 {
     uint32_t in_block = threadIdx.x >> c.lanes_log2;
     if (WAVE) in_block = __builtin_amdgcn_readfirstlane(in_block);
-    return static_cast<uint64_t>(blockIdx.x) * (kThreads >> c.lanes_log2) + in_block;
+    return (blockIdx.x - c.pad_blocks) * (THREADS >> c.lanes_log2) + in_block;
 }
 
-__device__ __forceinline__ uint64_t token_of(const Cut& c, uint64_t item, uint32_t* piece)
+// The rows of slots j0 .. j0 + K - 1 of a token; `rows` (none) for slots without one and behind the last.
+// The loads do not depend on how many slots there are (those behind the last repeat it): guarded one by one they
+// would also be waited for one by one.
+template <uint32_t K>
+__device__ __forceinline__ void load_slots(const int32_t* __restrict__ row_of_slot, uint32_t t, uint32_t j0, const MoveArgs& a,
+                                           uint32_t (&r)[K])
 {
-    if (c.pieces == 1) {
-        *piece = 0;
-        return item;
-    }
-    if (item >> 32) {
-        const uint64_t t = item / c.pieces;
-        *piece = static_cast<uint32_t>(item - t * c.pieces);
-        return t;
-    }
-    const uint32_t t = static_cast<uint32_t>(item) / c.pieces;
-    *piece = static_cast<uint32_t>(item) - t * c.pieces;
-    return t;
+    const int32_t* slots = row_of_slot + static_cast<uint64_t>(t) * a.topk;
+#pragma unroll
+    for (uint32_t j = 0; j < K; ++j) r[j] = static_cast<uint32_t>(slots[min(j0 + j, a.topk - 1)]);
+#pragma unroll
+    for (uint32_t j = 0; j < K; ++j)
+        if (j0 + j >= a.topk || r[j] > a.rows) r[j] = a.rows;
+}
+template <uint32_t K>
+__device__ __forceinline__ void load_weights(const float* __restrict__ weights, uint32_t t, uint32_t j0, const MoveArgs& a,
+                                             float (&w)[K])
+{
+    weights += static_cast<uint64_t>(t) * a.topk;
+#pragma unroll
+    for (uint32_t j = 0; j < K; ++j) w[j] = weights[min(j0 + j, a.topk - 1)];
 }
 
 // ---- dispatch: a row is read once and written `topk` times -----------------------------------
-template <typename Elem, bool WAVE>
-__global__ __launch_bounds__(kThreads) void route_dispatch_kernel(const MoveArgs a, const Cut c)
+// Workgroups of two waves, rows written through the caches: 0.239 ms for 16384 tokens, 8 slots, 4096 bf16 (1.1 GB
+// written, 5.3 TB/s in all; a plain copy reaches 5.0).  Larger workgroups or stores past the caches: 0.243 to 0.261; reading
+// by row, so that the writes run through the buffer in order: 0.34, the reads no longer come from memory once.
+template <typename Elem, uint32_t K, bool WAVE>
+__global__ __launch_bounds__(kMoveThreads) void route_dispatch_kernel(const Elem* __restrict__ x, Elem* __restrict__ out,
+                                                                      const int32_t* __restrict__ row_of_slot, const MoveArgs a,
+                                                                      const Cut c)
 {
-    if (blockIdx.x >= c.blocks) {
-        zero_padding<Elem>(a, c, blockIdx.x - c.blocks);
+    if (blockIdx.x < c.pad_blocks) {
+        zero_padding<Elem, kMoveThreads>(a, c, blockIdx.x);
         return;
     }
     constexpr uint32_t N = 16 / sizeof(Elem);
     const uint32_t lane = threadIdx.x & ((1u << c.lanes_log2) - 1);
-    const uint64_t step = static_cast<uint64_t>(c.blocks) * (kThreads >> c.lanes_log2);
-    for (uint64_t item = first_item<WAVE>(c); item < c.items; item += step) {
-        uint32_t piece;
-        const uint64_t t = token_of(c, item, &piece);
-        const uint32_t h = ((piece << c.lanes_log2) + lane) * N;
-        if (h >= a.hidden) continue;
-        const Elem* in = static_cast<const Elem*>(a.token_in) + t * a.ld_token_in + h;
-        Elem* out = static_cast<Elem*>(a.rows_out) + h;
-        const int32_t* slots = a.row_of_slot + t * a.topk;
-        if (h + N <= a.hidden) {
-            const RouteVec v = load_vec(in);
-            for (uint32_t j = 0; j < a.topk; ++j) {
-                const uint32_t r = static_cast<uint32_t>(slots[j]);
-                if (r < a.rows) store_vec(out + static_cast<uint64_t>(r) * a.ld_rows_out, v);
+    const uint32_t step = c.blocks * (kMoveThreads >> c.lanes_log2);
+    for (uint32_t item = first_item<kMoveThreads, WAVE>(c); item < c.items; item += step) {
+        const uint32_t t = item / c.pieces, piece = item - t * c.pieces;
+        const Elem* in = x + static_cast<uint64_t>(t) * a.ld_token_in;
+        const uint32_t v = (piece << c.lanes_log2) + lane;
+        RouteVec d = {0, 0, 0, 0};
+        if (v < c.vectors) d = load_vec(in + v * N);
+        for (uint32_t j0 = 0; j0 < a.topk; j0 += K) {
+            uint32_t r[K];
+            load_slots<K>(row_of_slot, t, j0, a, r);
+            if (v < c.vectors) {
+#pragma unroll
+                for (uint32_t j = 0; j < K; ++j)
+                    if (r[j] < a.rows) store_vec(out + r[j] * a.ld_rows_out + v * N, d);
             }
-        } else {
-            for (uint32_t j = 0; j < a.topk; ++j) {
-                const uint32_t r = static_cast<uint32_t>(slots[j]);
-                if (r >= a.rows) continue;
-                for (uint32_t i = 0; h + i < a.hidden; ++i) out[static_cast<uint64_t>(r) * a.ld_rows_out + i] = in[i];
+            for (uint32_t h = c.vectors * N + lane; piece == c.pieces - 1 && h < a.hidden; h += 1u << c.lanes_log2) {
+                const Elem e = in[h];
+#pragma unroll
+                for (uint32_t j = 0; j < K; ++j)
+                    if (r[j] < a.rows) out[r[j] * a.ld_rows_out + h] = e;
             }
         }
     }
 }
 
 // ---- combine: `topk` rows are read, one is written --------------------------------------------
-// Rows are loaded eight at a time before the first is used.  The sum is held in 32 bits and runs in
-// the order of the slots, one fused multiply-add each.
-template <typename T, bool WEIGHTED, bool WAVE>
-__global__ __launch_bounds__(kThreads) void route_combine_kernel(const MoveArgs a, const Cut c)
+// Up to eight rows' pieces are loaded before the first is used.  The sum is held in 32 bits and runs in the
+// order of the slots, one fused multiply-add each.  Workgroups of 16 waves, which read whole rows of up to 16 KiB
+// at about the same time, and loads past the caches: 0.205 ms for 16384 tokens, 8 slots, 4096 bf16 (5.9 TB/s); with
+// workgroups of 4 waves 0.214, with ordinary loads 0.231, with neither 0.24.  Where the rows fit the memory-side
+// cache ordinary loads win: 64 MiB of them 13.5 against 14 us.
+template <typename T, uint32_t K, bool MORE, bool WEIGHTED, bool WAVE, bool STREAM>
+__global__ __launch_bounds__(kSumThreads) void route_combine_kernel(const T* __restrict__ rows, T* __restrict__ out,
+                                                                    const int32_t* __restrict__ row_of_slot,
+                                                                    const float* __restrict__ weights, const MoveArgs a, const Cut c)
 {
     constexpr uint32_t N = 16 / sizeof(T);
-    constexpr uint32_t B = 8;
     const uint32_t lane = threadIdx.x & ((1u << c.lanes_log2) - 1);
-    const uint64_t step = static_cast<uint64_t>(c.blocks) * (kThreads >> c.lanes_log2);
-    for (uint64_t item = first_item<WAVE>(c); item < c.items; item += step) {
-        uint32_t piece;
-        const uint64_t t = token_of(c, item, &piece);
-        const uint32_t h = ((piece << c.lanes_log2) + lane) * N;
-        if (h >= a.hidden) continue;
-        const T* in = static_cast<const T*>(a.rows_in) + h;
-        T* out = static_cast<T*>(a.token_out) + t * a.ld_token_out + h;
-        const int32_t* slots = a.row_of_slot + t * a.topk;
-        const float* weights = WEIGHTED ? a.weights + t * a.topk : nullptr;
-        if (h + N <= a.hidden) {
+    const uint32_t step = c.blocks * (kSumThreads >> c.lanes_log2);
+    for (uint32_t item = first_item<kSumThreads, WAVE>(c); item < c.items; item += step) {
+        const uint32_t t = item / c.pieces, piece = item - t * c.pieces;
+        T* to = out + static_cast<uint64_t>(t) * a.ld_token_out;
+        const uint32_t v = (piece << c.lanes_log2) + lane;
+        uint32_t r[K];
+        float w[K];
+        load_slots<K>(row_of_slot, t, 0, a, r);
+        if (WEIGHTED) load_weights<K>(weights, t, 0, a, w);
+        if (v < c.vectors) {
             float acc[N];
 #pragma unroll
             for (uint32_t i = 0; i < N; ++i) acc[i] = 0.0f;
-            for (uint32_t j0 = 0; j0 < a.topk; j0 += B) {
-                RouteVec v[B];
-                uint32_t r[B];
+            for (uint32_t j0 = 0;;) {
+                RouteVec d[K];
 #pragma unroll
-                for (uint32_t j = 0; j < B; ++j) r[j] = j0 + j < a.topk ? static_cast<uint32_t>(slots[j0 + j]) : 0xFFFFFFFFu;
-#pragma unroll
-                for (uint32_t j = 0; j < B; ++j) {
-                    v[j] = RouteVec{0, 0, 0, 0};
-                    if (r[j] < a.rows) v[j] = load_vec(in + static_cast<uint64_t>(r[j]) * a.ld_rows_in);
+                for (uint32_t j = 0; j < K; ++j) {
+                    d[j] = RouteVec{0, 0, 0, 0};
+                    if (r[j] < a.rows) d[j] = get<STREAM>(rows + r[j] * a.ld_rows_in + v * N);
                 }
 #pragma unroll
-                for (uint32_t j = 0; j < B; ++j) {
+                for (uint32_t j = 0; j < K; ++j) {
                     if (r[j] >= a.rows) continue;
-                    const float w = WEIGHTED ? weights[j0 + j] : 1.0f;
-                    const RouteElems<T> e = as_elems<T>(v[j]);
+                    const RouteElems<T> e = as_elems<T>(d[j]);
 #pragma unroll
-                    for (uint32_t i = 0; i < N; ++i) acc[i] = WEIGHTED ? fmaf(w, to_f32(e.e[i]), acc[i]) : acc[i] + to_f32(e.e[i]);
+                    for (uint32_t i = 0; i < N; ++i) acc[i] = WEIGHTED ? fmaf(w[j], to_f32(e.e[i]), acc[i]) : acc[i] + to_f32(e.e[i]);
                 }
+                j0 += K;
+                if (!MORE || j0 >= a.topk) break;
+                load_slots<K>(row_of_slot, t, j0, a, r);
+                if (WEIGHTED) load_weights<K>(weights, t, j0, a, w);
             }
             RouteElems<T> o;
 #pragma unroll
             for (uint32_t i = 0; i < N; ++i) o.e[i] = static_cast<T>(acc[i]);
-            store_vec(out, as_vec(o));
-        } else {
-            for (uint32_t i = 0; h + i < a.hidden; ++i) {
-                float acc = 0.0f;
-                for (uint32_t j = 0; j < a.topk; ++j) {
-                    const uint32_t r = static_cast<uint32_t>(slots[j]);
-                    if (r >= a.rows) continue;
-                    const float x = to_f32(in[static_cast<uint64_t>(r) * a.ld_rows_in + i]);
-                    acc = WEIGHTED ? fmaf(weights[j], x, acc) : acc + x;
-                }
-                out[i] = static_cast<T>(acc);
+            put<STREAM>(to + v * N, as_vec(o));
+        }
+        for (uint32_t h = c.vectors * N + lane; piece == c.pieces - 1 && h < a.hidden; h += 1u << c.lanes_log2) {
+            float acc = 0.0f;
+            for (uint32_t j = 0; j < a.topk; ++j) {
+                uint32_t r[1];
+                load_slots<1>(row_of_slot, t, j, a, r);
+                if (r[0] >= a.rows) continue;
+                const float x = to_f32(rows[r[0] * a.ld_rows_in + h]);
+                acc = WEIGHTED ? fmaf(weights[static_cast<uint64_t>(t) * a.topk + j], x, acc) : acc + x;
             }
+            to[h] = static_cast<T>(acc);
         }
     }
 }
 
 // ---- combine's gradient ----------------------------------------------------------------------
-// One pass: a piece of out_grad is read once, and for every slot the piece of its row is read for the
-// dot product and the weighted piece written.  A token belongs to one group of lanes, which walks
-// its row; the lanes' partial dot products are added by a fixed tree at the end, so
-// results are the same every time.
-template <typename T, uint32_t K, bool WAVE>
-__global__ __launch_bounds__(kThreads) void route_combine_backward_kernel(const MoveArgs a, const Cut c)
+// For K slots at a time: a piece of out_grad is read, and for every slot the piece of its row is read for the dot
+// product and the weighted piece written.  token_waves waves of a workgroup share a token; the lanes' partial dot
+// products are added by a fixed tree, the waves' in order, so results are the same every time.  Reads and writes
+// come in equal parts, past the caches where they are large: 0.445 ms for 16384 tokens, 8 slots, 4096 bf16 (5.3 TB/s; a
+// plain copy 5.0).  One wave for each token: 0.463; through the caches: 0.468.
+
+// Sums of K values over a wave, M = 32.  While there are several values left, a step hands half of them to the
+// other half of the lanes.  Lane l returns the sum of value l / (64 / K).
+template <uint32_t K, uint32_t M>
+__device__ __forceinline__ float sums_over_wave(const float (&v)[K])
 {
-    if (blockIdx.x >= c.blocks) {
-        zero_padding<T>(a, c, blockIdx.x - c.blocks);
+    if constexpr (M == 0) {
+        return v[0];
+    } else if constexpr (K == 1) {
+        const float both[1] = {v[0] + __shfl_xor(v[0], static_cast<int>(M))};
+        return sums_over_wave<1, M / 2>(both);
+    } else {
+        const bool upper = threadIdx.x & M;
+        float half[K / 2];
+#pragma unroll
+        for (uint32_t j = 0; j < K / 2; ++j) {
+            const float give = upper ? v[j] : v[j + K / 2];
+            const float keep = upper ? v[j + K / 2] : v[j];
+            half[j] = keep + __shfl_xor(give, static_cast<int>(M));
+        }
+        return sums_over_wave<K / 2, M / 2>(half);
+    }
+}
+
+template <typename T, uint32_t K, bool WAVE, bool STREAM>
+__global__ __launch_bounds__(kSumThreads) void route_combine_backward_kernel(const T* __restrict__ rows, const T* __restrict__ out_grad,
+                                                                             T* __restrict__ rows_grad,
+                                                                             const int32_t* __restrict__ row_of_slot,
+                                                                             const float* __restrict__ weights, const MoveArgs a,
+                                                                             const Cut c)
+{
+    if (blockIdx.x < c.pad_blocks) {
+        zero_padding<T, kSumThreads>(a, c, blockIdx.x);
         return;
     }
     constexpr uint32_t N = 16 / sizeof(T);
-    constexpr uint32_t B = K < 8 ? K : 8;
-    const uint32_t lanes = 1u << c.lanes_log2;
-    const uint32_t lane = threadIdx.x & (lanes - 1);
-    const uint64_t step = static_cast<uint64_t>(c.blocks) * (kThreads >> c.lanes_log2);
-    for (uint64_t t = first_item<WAVE>(c); t < c.items; t += step) {
-        const int32_t* slots = a.row_of_slot + t * a.topk;
-        const float* weights = a.weights + t * a.topk;
-        const T* grad = static_cast<const T*>(a.token_in) + t * a.ld_token_in;
-        float dot[K];
+    __shared__ float partial[2][kSumThreads / 64][K];
+    const uint32_t lanes = 1u << c.lanes_log2, lane = threadIdx.x & (lanes - 1);
+    const uint32_t per_block = kSumThreads >> c.lanes_log2;
+    uint32_t item = first_item<kSumThreads, WAVE>(c);
+    uint32_t half = 0;
+    // the whole workgroup leaves together: its first item is what counts
+    for (uint32_t base = (blockIdx.x - c.pad_blocks) * per_block; base < c.items; base += c.blocks * per_block, item += c.blocks * per_block) {
+        const uint32_t t = item / c.token_waves, share = item - t * c.token_waves;
+        for (uint32_t j0 = 0; j0 < a.topk; j0 += K) {
+            float dot[K];
 #pragma unroll
-        for (uint32_t j = 0; j < K; ++j) dot[j] = 0.0f;
-        for (uint32_t h = lane * N; h < a.hidden; h += lanes * N) {
-            const T* in = static_cast<const T*>(a.rows_in) + h;
-            T* out = static_cast<T*>(a.rows_out) + h;
-            if (h + N <= a.hidden) {
-                const RouteElems<T> ge = as_elems<T>(load_vec(grad + h));
+            for (uint32_t j = 0; j < K; ++j) dot[j] = 0.0f;
+            if (item < c.items) {
+                uint32_t r[K];
+                float w[K];
+                load_slots<K>(row_of_slot, t, j0, a, r);
+                load_weights<K>(weights, t, j0, a, w);
+                const T* grad = out_grad + static_cast<uint64_t>(t) * a.ld_token_in;
+                for (uint32_t v = (share << c.lanes_log2) + lane; v < c.vectors; v += c.token_waves << c.lanes_log2) {
+                    const RouteElems<T> ge = as_elems<T>(get<STREAM>(grad + v * N));
+                    RouteVec d[K];
 #pragma unroll
-                for (uint32_t j0 = 0; j0 < K; j0 += B) {
-                    RouteVec v[B];
-                    uint32_t r[B];
-#pragma unroll
-                    for (uint32_t j = 0; j < B; ++j) r[j] = j0 + j < a.topk ? static_cast<uint32_t>(slots[j0 + j]) : 0xFFFFFFFFu;
-#pragma unroll
-                    for (uint32_t j = 0; j < B; ++j) {
-                        v[j] = RouteVec{0, 0, 0, 0};
-                        if (r[j] < a.rows) v[j] = load_vec(in + static_cast<uint64_t>(r[j]) * a.ld_rows_in);
+                    for (uint32_t j = 0; j < K; ++j) {
+                        d[j] = RouteVec{0, 0, 0, 0};
+                        if (r[j] < a.rows) d[j] = get<STREAM>(rows + r[j] * a.ld_rows_in + v * N);
                     }
 #pragma unroll
-                    for (uint32_t j = 0; j < B; ++j) {
+                    for (uint32_t j = 0; j < K; ++j) {
                         if (r[j] >= a.rows) continue;
-                        const float w = weights[j0 + j];
-                        const RouteElems<T> e = as_elems<T>(v[j]);
+                        const RouteElems<T> e = as_elems<T>(d[j]);
                         RouteElems<T> o;
 #pragma unroll
                         for (uint32_t i = 0; i < N; ++i) {
                             const float g = to_f32(ge.e[i]);
-                            dot[j0 + j] = fmaf(g, to_f32(e.e[i]), dot[j0 + j]);
-                            o.e[i] = static_cast<T>(w * g);
+                            dot[j] = fmaf(g, to_f32(e.e[i]), dot[j]);
+                            o.e[i] = static_cast<T>(w[j] * g);
                         }
-                        store_vec(out + static_cast<uint64_t>(r[j]) * a.ld_rows_out, as_vec(o));
+                        put<STREAM>(rows_grad + r[j] * a.ld_rows_out + v * N, as_vec(o));
                     }
+                }
+                for (uint32_t h = c.vectors * N + lane; share == c.token_waves - 1 && h < a.hidden; h += lanes) {
+                    const float g = to_f32(grad[h]);
+#pragma unroll
+                    for (uint32_t j = 0; j < K; ++j) {
+                        if (r[j] >= a.rows) continue;
+                        dot[j] = fmaf(g, to_f32(rows[r[j] * a.ld_rows_in + h]), dot[j]);
+                        rows_grad[r[j] * a.ld_rows_out + h] = static_cast<T>(w[j] * g);
+                    }
+                }
+            }
+            float* sums = a.weights_grad + static_cast<uint64_t>(t) * a.topk + j0;
+            if (WAVE) {
+                constexpr uint32_t kLanesPerSlot = 64 / K;
+                const float d = sums_over_wave<K, 32>(dot);
+                const uint32_t j = lane / kLanesPerSlot;
+                const bool first_lane = lane % kLanesPerSlot == 0;
+                const bool writes = first_lane && j0 + j < a.topk && item < c.items;
+                if (c.token_waves == 1) {
+                    if (writes) sums[j] = d;
+                } else {
+                    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+                    if (first_lane) partial[half][wave][j] = d;
+                    __syncthreads();
+                    if (share == 0 && writes) {
+                        float sum = d;
+                        for (uint32_t i = 1; i < c.token_waves; ++i) sum += partial[half][wave + i][j];
+                        sums[j] = sum;
+                    }
+                    half ^= 1;  // the next round writes the other half: one barrier a round is enough
                 }
             } else {
 #pragma unroll
                 for (uint32_t j = 0; j < K; ++j) {
-                    const uint32_t r = j < a.topk ? static_cast<uint32_t>(slots[j]) : 0xFFFFFFFFu;
-                    if (r >= a.rows) continue;
-                    const float w = weights[j];
-                    for (uint32_t i = 0; h + i < a.hidden; ++i) {
-                        const float g = to_f32(grad[h + i]);
-                        dot[j] = fmaf(g, to_f32(in[static_cast<uint64_t>(r) * a.ld_rows_in + i]), dot[j]);
-                        out[static_cast<uint64_t>(r) * a.ld_rows_out + i] = static_cast<T>(w * g);
-                    }
+                    float d = dot[j];
+                    for (uint32_t m = lanes >> 1; m > 0; m >>= 1) d += __shfl_xor(d, static_cast<int>(m), static_cast<int>(lanes));
+                    if (item < c.items && j0 + j < a.topk && lane == (j & (lanes - 1))) sums[j] = d;
                 }
             }
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < K; ++j) {
-            float d = dot[j];
-            for (uint32_t m = lanes >> 1; m > 0; m >>= 1) d += __shfl_xor(d, static_cast<int>(m), static_cast<int>(lanes));
-            if (j < a.topk && lane == (j & (lanes - 1))) a.weights_grad[t * a.topk + j] = d;
         }
     }
 }
 
-}  // namespace
-
-int launch_route_dispatch(int element_bytes, const MoveArgs& a, int num_cus, hipStream_t s)
+// Calls f with the number of slots a kernel takes at a time, and whether there are more.
+template <typename F>
+void with_slots(uint32_t topk, F&& f)
 {
-    (void)num_cus;
-    const Cut c = cut_rows(a, element_bytes, false, true);
-    const dim3 grid(c.blocks + c.pad_blocks), block(kThreads);
-    if (grid.x == 0) return MRS_OK;
-    const auto go = [&](auto elem) {
-        using E = decltype(elem);
-        if (c.lanes_log2 == 6)
-            hipLaunchKernelGGL((route_dispatch_kernel<E, true>), grid, block, 0, s, a, c);
-        else
-            hipLaunchKernelGGL((route_dispatch_kernel<E, false>), grid, block, 0, s, a, c);
-    };
-    if (element_bytes == 1)
-        go(uint8_t{});
-    else if (element_bytes == 2)
-        go(uint16_t{});
+    if (topk <= 4)
+        f(std::integral_constant<uint32_t, 4>{}, std::false_type{});
+    else if (topk <= 8)
+        f(std::integral_constant<uint32_t, 8>{}, std::false_type{});
     else
-        go(uint32_t{});
+        f(std::integral_constant<uint32_t, 8>{}, std::true_type{});
+}
+
+template <typename E>
+int start_dispatch(const MoveArgs& a, hipStream_t s)
+{
+    Cut c;
+    if (int rc = cut_rows(a, sizeof(E), kMoveThreads, false, true, &c)) return rc;
+    const dim3 grid(c.blocks + c.pad_blocks), block(kMoveThreads);
+    with_slots(a.topk, [&](auto k, auto) {
+        constexpr uint32_t K = decltype(k)::value;
+        const E* x = static_cast<const E*>(a.token_in);
+        E* rows = static_cast<E*>(a.rows_out);
+        if (c.lanes_log2 == 6)
+            hipLaunchKernelGGL((route_dispatch_kernel<E, K, true>), grid, block, 0, s, x, rows, a.row_of_slot, a, c);
+        else
+            hipLaunchKernelGGL((route_dispatch_kernel<E, K, false>), grid, block, 0, s, x, rows, a.row_of_slot, a, c);
+    });
     MRS_CHECK_LAUNCH("route_dispatch_kernel");
     return MRS_OK;
 }
 
-template <typename T>
-static void start_combine(const MoveArgs& a, hipStream_t s)
+template <typename T, bool WEIGHTED>
+int start_combine(const MoveArgs& a, hipStream_t s)
 {
-    const Cut c = cut_rows(a, sizeof(T), false, false);
-    const dim3 grid(c.blocks), block(kThreads);
-    if (grid.x == 0) return;
-    const bool wave = c.lanes_log2 == 6;
-    if (a.weights) {
-        if (wave)
-            hipLaunchKernelGGL((route_combine_kernel<T, true, true>), grid, block, 0, s, a, c);
+    Cut c;
+    if (int rc = cut_rows(a, sizeof(T), kSumThreads, false, false, &c)) return rc;
+    const dim3 grid(c.blocks), block(kSumThreads);
+    const bool stream = a.tokens * a.topk * a.hidden * sizeof(T) >= kStreamBytes;
+    // a loop for more than eight slots costs the others 1 %
+    with_slots(a.topk, [&](auto k, auto more) {
+        constexpr uint32_t K = decltype(k)::value;
+        constexpr bool MORE = decltype(more)::value;
+        const T* rows = static_cast<const T*>(a.rows_in);
+        T* out = static_cast<T*>(a.token_out);
+        if (c.lanes_log2 < 6)
+            hipLaunchKernelGGL((route_combine_kernel<T, K, MORE, WEIGHTED, false, false>), grid, block, 0, s, rows, out, a.row_of_slot, a.weights, a, c);
+        else if (!stream)
+            hipLaunchKernelGGL((route_combine_kernel<T, K, MORE, WEIGHTED, true, false>), grid, block, 0, s, rows, out, a.row_of_slot, a.weights, a, c);
         else
-            hipLaunchKernelGGL((route_combine_kernel<T, true, false>), grid, block, 0, s, a, c);
-    } else {
-        if (wave)
-            hipLaunchKernelGGL((route_combine_kernel<T, false, true>), grid, block, 0, s, a, c);
-        else
-            hipLaunchKernelGGL((route_combine_kernel<T, false, false>), grid, block, 0, s, a, c);
-    }
-}
-
-int launch_route_combine(int type, const MoveArgs& a, int num_cus, hipStream_t s)
-{
-    (void)num_cus;
-    if (type == MRS_TYPE_F32)
-        start_combine<float>(a, s);
-    else if (type == MRS_TYPE_F16)
-        start_combine<_Float16>(a, s);
-    else
-        start_combine<__bf16>(a, s);
+            hipLaunchKernelGGL((route_combine_kernel<T, K, MORE, WEIGHTED, true, true>), grid, block, 0, s, rows, out, a.row_of_slot, a.weights, a, c);
+    });
     MRS_CHECK_LAUNCH("route_combine_kernel");
     return MRS_OK;
 }
 
 template <typename T>
-static void start_combine_backward(const MoveArgs& a, hipStream_t s)
+int start_combine_backward(const MoveArgs& a, hipStream_t s)
 {
-    const Cut c = cut_rows(a, sizeof(T), true, true);
-    const dim3 grid(c.blocks + c.pad_blocks), block(kThreads);
-    if (grid.x == 0) return;
-    const auto go = [&](auto k) {
+    Cut c;
+    if (int rc = cut_rows(a, sizeof(T), kSumThreads, true, true, &c)) return rc;
+    const dim3 grid(c.blocks + c.pad_blocks), block(kSumThreads);
+    const bool stream = 2 * a.tokens * a.topk * a.hidden * sizeof(T) >= kStreamBytes;  // read and written
+    with_slots(a.topk, [&](auto k, auto) {
         constexpr uint32_t K = decltype(k)::value;
-        if (c.lanes_log2 == 6)
-            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, true>), grid, block, 0, s, a, c);
+        const T* rows = static_cast<const T*>(a.rows_in);
+        const T* grad = static_cast<const T*>(a.token_in);
+        T* out = static_cast<T*>(a.rows_out);
+        if (c.lanes_log2 < 6)
+            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, false, false>), grid, block, 0, s, rows, grad, out, a.row_of_slot, a.weights, a, c);
+        else if (!stream)
+            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, true, false>), grid, block, 0, s, rows, grad, out, a.row_of_slot, a.weights, a, c);
         else
-            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, false>), grid, block, 0, s, a, c);
-    };
-    if (a.topk <= 2)
-        go(std::integral_constant<uint32_t, 2>{});
-    else if (a.topk <= 4)
-        go(std::integral_constant<uint32_t, 4>{});
-    else if (a.topk <= 8)
-        go(std::integral_constant<uint32_t, 8>{});
-    else if (a.topk <= 16)
-        go(std::integral_constant<uint32_t, 16>{});
-    else
-        go(std::integral_constant<uint32_t, 32>{});
-}
-
-int launch_route_combine_backward(int type, const MoveArgs& a, int num_cus, hipStream_t s)
-{
-    (void)num_cus;
-    if (type == MRS_TYPE_F32)
-        start_combine_backward<float>(a, s);
-    else if (type == MRS_TYPE_F16)
-        start_combine_backward<_Float16>(a, s);
-    else
-        start_combine_backward<__bf16>(a, s);
+            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, true, true>), grid, block, 0, s, rows, grad, out, a.row_of_slot, a.weights, a, c);
+    });
     MRS_CHECK_LAUNCH("route_combine_backward_kernel");
     return MRS_OK;
+}
+
+}  // namespace
+
+int launch_route_dispatch(int element_bytes, const MoveArgs& a, int, hipStream_t s)
+{
+    if (element_bytes == 1) return start_dispatch<uint8_t>(a, s);
+    if (element_bytes == 2) return start_dispatch<uint16_t>(a, s);
+    return start_dispatch<uint32_t>(a, s);
+}
+
+int launch_route_combine(int type, const MoveArgs& a, int, hipStream_t s)
+{
+    if (type == MRS_TYPE_F32) return a.weights ? start_combine<float, true>(a, s) : start_combine<float, false>(a, s);
+    if (type == MRS_TYPE_F16) return a.weights ? start_combine<_Float16, true>(a, s) : start_combine<_Float16, false>(a, s);
+    return a.weights ? start_combine<__bf16, true>(a, s) : start_combine<__bf16, false>(a, s);
+}
+
+int launch_route_combine_backward(int type, const MoveArgs& a, int, hipStream_t s)
+{
+    if (type == MRS_TYPE_F32) return start_combine_backward<float>(a, s);
+    if (type == MRS_TYPE_F16) return start_combine_backward<_Float16>(a, s);
+    return start_combine_backward<__bf16>(a, s);
 }
 
 }  // namespace mrs
