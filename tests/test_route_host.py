@@ -1,7 +1,6 @@
 """Token routing without a GPU: the sizes the library reports, what it refuses, and that the definitions
 the GPU tests compare with have the derivatives they say."""
 import ctypes
-import types
 
 import pytest
 import torch
@@ -77,7 +76,7 @@ def test_null_arguments_are_refused():
 def _plan_on_the_cpu(tokens=4, experts=8, topk=2):
     """The Python checks alone: a plan without a handle, on CPU tensors."""
     plan = object.__new__(mrs.RoutePlan)
-    plan.ctx, plan.lib, plan._h = types.SimpleNamespace(device=torch.device("cpu")), _lib.load_library(), None
+    plan.device, plan.lib, plan._h = torch.device("cpu"), _lib.load_library(), None
     plan.tokens, plan.experts, plan.topk, plan.max_rows = tokens, experts, topk, tokens * topk
     return plan
 
@@ -85,7 +84,7 @@ def _plan_on_the_cpu(tokens=4, experts=8, topk=2):
 def test_tensor_checks(monkeypatch):
     from wgpu_morton_code_radix_sort_test_amd import api
 
-    monkeypatch.setattr(api, "_stream", lambda stream: None)
+    monkeypatch.setattr(api, "_raw_stream", lambda index: 0)
     plan = _plan_on_the_cpu()
     route = plan.new_map()
     x, rows = torch.zeros(4, 6), torch.zeros(8, 6)
@@ -122,7 +121,7 @@ def test_tensor_checks(monkeypatch):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was taken")
-    plan.ctx.device = torch.device("cuda", 0)  # tensors elsewhere than the plan
+    plan.device = torch.device("cuda", 0)  # tensors elsewhere than the plan
     with pytest.raises(ValueError, match="is on"):
         plan.dispatch(x, route)
 

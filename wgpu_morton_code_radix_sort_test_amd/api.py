@@ -407,6 +407,8 @@ class SortPlan:
 # MRS_TYPE_* of the element types rows can have
 _ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _TYPE_8BIT = 3
+# The current stream's handle without the Stream object around it, which takes 3 us to make.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 @dataclass(frozen=True)
@@ -432,6 +434,7 @@ class RoutePlan:
         self._h = None
         self.ctx = ctx
         self.lib = ctx.lib
+        self.device = ctx.device
         for name, v in (("tokens", tokens), ("capacity", capacity)):
             if v < 0:
                 raise ValueError(f"{name} must not be negative")
@@ -455,28 +458,30 @@ class RoutePlan:
         except Exception:
             pass
 
-    # ---- checks --------------------------------------------------------------------
+    # ---- checks: a call takes a few microseconds of host time, most of them here -----------------
     def _on_device(self, t, name):
-        if t.device != self.ctx.device:
-            raise ValueError(f"{name} is on {t.device}, the plan on {self.ctx.device}")
+        if t.device != self.device:
+            raise ValueError(f"{name} is on {t.device}, the plan on {self.device}")
 
     def _rows(self, t, name, rows, hidden, dtype):
         """Pointer and row stride of a matrix whose rows are contiguous."""
-        self._on_device(t, name)
-        if t.dim() != 2 or t.size(0) != rows or t.size(1) != hidden:
+        if t.device != self.device:
+            self._on_device(t, name)
+        if t.shape != (rows, hidden):
             raise ValueError(f"{name} must have shape [{rows}, {hidden}], not {list(t.shape)}")
         if t.dtype != dtype:
             raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-        ld = t.stride(0)
-        if hidden > 1 and t.stride(1) != 1:
+        ld, step = t.stride()
+        if step != 1 and hidden > 1:
             raise ValueError(f"the rows of {name} must be contiguous")
         if rows <= 1 and ld < hidden:
             ld = hidden
         return t.data_ptr(), ld
 
     def _per_slot(self, t, name, tokens, dtype):
-        self._on_device(t, name)
-        if t.dtype != dtype or t.dim() != 2 or t.size(0) != tokens or t.size(1) != self.topk or not t.is_contiguous():
+        if t.device != self.device:
+            self._on_device(t, name)
+        if t.dtype != dtype or t.shape != (tokens, self.topk) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape [{tokens}, {self.topk}]")
         return t.data_ptr()
 
@@ -485,15 +490,22 @@ class RoutePlan:
             raise ValueError(f"{name} must have two dimensions, not {t.dim()}")
         return t.size(0)
 
-    def _map(self, route, tokens):
-        rows = route.slot_of_row.numel()
-        for t, name, least in ((route.row_of_slot, "row_of_slot", tokens * self.topk), (route.slot_of_row, "slot_of_row", 0),
-                               (route.counts, "counts", self.experts), (route.offsets, "offsets", self.experts + 1)):
+    def _indices(self, t, name, least):
+        if t.device != self.device:
             self._on_device(t, name)
-            if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < least:
-                raise ValueError(f"{name} must be a contiguous int32 tensor of at least {least} elements")
-        return ctypes.byref(_lib.RouteMapStruct(route.row_of_slot.data_ptr(), route.slot_of_row.data_ptr(),
-                                                route.counts.data_ptr(), route.offsets.data_ptr(), rows)), rows
+        if t.dtype != torch.int32 or t.numel() < least or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor of at least {least} elements")
+        return t.data_ptr()
+
+    def _map(self, route, tokens):
+        return _lib.RouteMapStruct(self._indices(route.row_of_slot, "row_of_slot", tokens * self.topk),
+                                   self._indices(route.slot_of_row, "slot_of_row", 0),
+                                   self._indices(route.counts, "counts", self.experts),
+                                   self._indices(route.offsets, "offsets", self.experts + 1),
+                                   route.slot_of_row.numel()), route.slot_of_row.numel()
+
+    def _on_stream(self, stream):
+        return _raw_stream(self.device.index) if stream is None else stream.cuda_stream
 
     def _row_type(self, t, name, eight_bits=False):
         if t.dim() != 2:
@@ -523,7 +535,7 @@ class RoutePlan:
     def new_map(self, tokens=None):
         """An unwritten RouteMap for `order` calls of `tokens` tokens (the plan's, by default)."""
         tokens = self.tokens if tokens is None else tokens
-        make = lambda *shape: torch.empty(shape, dtype=torch.int32, device=self.ctx.device)  # noqa: E731
+        make = lambda *shape: torch.empty(shape, dtype=torch.int32, device=self.device)  # noqa: E731
         return RouteMap(make(tokens, self.topk), make(self.max_rows), make(self.experts), make(self.experts + 1))
 
     def select(self, scores, bias=None, ids_out=None, weights_out=None, stream=None):
@@ -531,13 +543,13 @@ class RoutePlan:
         [tokens, topk], from scores [tokens, experts] (float32, float16 or bfloat16)."""
         tokens, kind, ptr, ld = self._scores(scores)
         if ids_out is None:
-            ids_out = torch.empty((tokens, self.topk), dtype=torch.int32, device=self.ctx.device)
+            ids_out = torch.empty((tokens, self.topk), dtype=torch.int32, device=self.device)
         if weights_out is None:
-            weights_out = torch.empty((tokens, self.topk), dtype=torch.float32, device=self.ctx.device)
+            weights_out = torch.empty((tokens, self.topk), dtype=torch.float32, device=self.device)
         _lib.check(
             self.lib.mrs_route_select(self._h, tokens, ptr, ld, kind, self._bias(bias),
                                       self._per_slot(ids_out, "ids_out", tokens, torch.int32),
-                                      self._per_slot(weights_out, "weights_out", tokens, torch.float32), _stream(stream))
+                                      self._per_slot(weights_out, "weights_out", tokens, torch.float32), self._on_stream(stream))
         )
         return ids_out, weights_out
 
@@ -545,13 +557,13 @@ class RoutePlan:
         """`mrs_route_select_backward`: the gradient of `scores`, of their type, from that of the weights."""
         tokens, kind, ptr, ld = self._scores(scores)
         if scores_grad_out is None:
-            scores_grad_out = torch.empty((tokens, self.experts), dtype=scores.dtype, device=self.ctx.device)
+            scores_grad_out = scores.new_empty((tokens, self.experts))
         grad_ptr, grad_ld = self._rows(scores_grad_out, "scores_grad_out", tokens, self.experts, scores.dtype)
         _lib.check(
             self.lib.mrs_route_select_backward(self._h, tokens, ptr, ld, kind, self._bias(bias),
                                                self._per_slot(ids, "ids", tokens, torch.int32),
                                                self._per_slot(weights_grad, "weights_grad", tokens, torch.float32),
-                                               grad_ptr, grad_ld, _stream(stream))
+                                               grad_ptr, grad_ld, self._on_stream(stream))
         )
         return scores_grad_out
 
@@ -563,7 +575,7 @@ class RoutePlan:
         if map_out is None:
             map_out = self.new_map(tokens)
         raw, _ = self._map(map_out, tokens)
-        _lib.check(self.lib.mrs_route_order(self._h, tokens, ids_ptr, raw, _stream(stream)))
+        _lib.check(self.lib.mrs_route_order(self._h, tokens, ids_ptr, raw, self._on_stream(stream)))
         return map_out
 
     def dispatch(self, x, route, rows_out=None, stream=None):
@@ -574,9 +586,9 @@ class RoutePlan:
         raw, rows = self._map(route, tokens)
         x_ptr, ld_x = self._rows(x, "x", tokens, hidden, x.dtype)
         if rows_out is None:
-            rows_out = torch.empty((rows, hidden), dtype=x.dtype, device=self.ctx.device)
+            rows_out = x.new_empty((rows, hidden))
         out_ptr, ld_out = self._rows(rows_out, "rows_out", rows, hidden, x.dtype)
-        _lib.check(self.lib.mrs_route_dispatch(self._h, tokens, raw, kind, hidden, x_ptr, ld_x, out_ptr, ld_out, _stream(stream)))
+        _lib.check(self.lib.mrs_route_dispatch(self._h, tokens, raw, kind, hidden, x_ptr, ld_x, out_ptr, ld_out, self._on_stream(stream)))
         return rows_out
 
     def dispatch_backward(self, rows_grad, route, x_grad_out=None, tokens=None, stream=None):
@@ -587,11 +599,11 @@ class RoutePlan:
         raw, rows = self._map(route, tokens)
         in_ptr, ld_in = self._rows(rows_grad, "rows_grad", rows, hidden, rows_grad.dtype)
         if x_grad_out is None:
-            x_grad_out = torch.empty((tokens, hidden), dtype=rows_grad.dtype, device=self.ctx.device)
+            x_grad_out = rows_grad.new_empty((tokens, hidden))
         out_ptr, ld_out = self._rows(x_grad_out, "x_grad_out", tokens, hidden, rows_grad.dtype)
         _lib.check(
             self.lib.mrs_route_dispatch_backward(self._h, tokens, raw, kind, hidden, in_ptr, ld_in, out_ptr, ld_out,
-                                                 _stream(stream))
+                                                 self._on_stream(stream))
         )
         return x_grad_out
 
@@ -602,12 +614,12 @@ class RoutePlan:
         raw, count = self._map(route, tokens)
         in_ptr, ld_in = self._rows(rows, "rows", count, hidden, rows.dtype)
         if out is None:
-            out = torch.empty((tokens, hidden), dtype=rows.dtype, device=self.ctx.device)
+            out = rows.new_empty((tokens, hidden))
         out_ptr, ld_out = self._rows(out, "out", tokens, hidden, rows.dtype)
         _lib.check(
             self.lib.mrs_route_combine(self._h, tokens, raw, kind, hidden, in_ptr, ld_in,
                                        self._per_slot(weights, "weights", tokens, torch.float32), out_ptr, ld_out,
-                                       _stream(stream))
+                                       self._on_stream(stream))
         )
         return out
 
@@ -620,15 +632,15 @@ class RoutePlan:
         grad_ptr, ld_grad = self._rows(out_grad, "out_grad", tokens, hidden, rows.dtype)
         in_ptr, ld_in = self._rows(rows, "rows", count, hidden, rows.dtype)
         if drows_out is None:
-            drows_out = torch.empty((count, hidden), dtype=rows.dtype, device=self.ctx.device)
+            drows_out = rows.new_empty((count, hidden))
         if dweights_out is None:
-            dweights_out = torch.empty((tokens, self.topk), dtype=torch.float32, device=self.ctx.device)
+            dweights_out = weights.new_empty((tokens, self.topk))
         out_ptr, ld_out = self._rows(drows_out, "drows_out", count, hidden, rows.dtype)
         _lib.check(
             self.lib.mrs_route_combine_backward(self._h, tokens, raw, kind, hidden, grad_ptr, ld_grad, in_ptr, ld_in,
                                                 self._per_slot(weights, "weights", tokens, torch.float32), out_ptr, ld_out,
                                                 self._per_slot(dweights_out, "dweights_out", tokens, torch.float32),
-                                                _stream(stream))
+                                                self._on_stream(stream))
         )
         return drows_out, dweights_out
 

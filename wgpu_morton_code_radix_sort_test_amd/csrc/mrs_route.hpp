@@ -89,6 +89,14 @@ typedef RouteVec RouteVecLoose __attribute__((aligned(1)));
 __device__ __forceinline__ RouteVec load_vec(const void* p) { return *static_cast<const RouteVecLoose*>(p); }
 __device__ __forceinline__ void store_vec(void* p, RouteVec v) { *static_cast<RouteVecLoose*>(p) = v; }
 
+// LDS written by some lanes of a wave is read by others: the accesses stay in order on the device, and this keeps the
+// compiler from moving them across.
+__device__ __forceinline__ void wave_lds_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Conversions; to fewer bits round to nearest even.
 template <typename T>
 __device__ __forceinline__ float to_f32(T v)

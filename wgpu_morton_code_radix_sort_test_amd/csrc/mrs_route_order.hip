@@ -21,15 +21,16 @@ constexpr uint32_t kWaves = 16;
 constexpr uint32_t kThreads = kWaves * 64;
 constexpr uint32_t kMaxExperts = MRS_ROUTE_MAX_EXPERTS;
 static_assert(kMaxExperts <= kThreads, "one thread per expert in the scans");
-constexpr uint32_t kSmallR = 8;
-constexpr uint32_t kSmallSlots = kThreads * kSmallR;
+constexpr uint32_t kSmallSlots = kThreads * 8;
 constexpr uint32_t kTileR = 4;
 constexpr uint32_t kTileSlots = kThreads * kTileR;
 
 struct OrderShared {
-    uint16_t wave_count[kWaves][kMaxExperts];  // slots per wave, then those of the waves before
+    alignas(4) uint16_t wave_count[kWaves][kMaxExperts];  // slots per wave, then those of the waves before
     uint32_t row[kMaxExperts];                 // first row of the expert in this tile
     uint32_t room[kMaxExperts];                // rows it may still take
+    uint32_t fill[kMaxExperts];                // first row of its segment without a slot
+    uint32_t fill_end[kMaxExperts];
     uint32_t wave_sum[kWaves];
 };
 
@@ -70,31 +71,42 @@ __device__ __forceinline__ uint32_t block_exclusive_scan(uint32_t v, uint32_t* w
 
 __device__ __forceinline__ uint32_t round_up_to(uint32_t v, uint32_t a) { return (v + a - 1) / a * a; }
 
-// Loads a tile's experts (`experts` where a slot has none) and ranks them inside their waves; the
-// waves' counters must be zero.
+// The experts of a tile's slots, `experts` where a slot has none.  A wave takes 64 * R neighbouring slots.
 template <uint32_t R>
-__device__ __forceinline__ void rank_in_waves(const OrderArgs& a, OrderShared& sh, uint64_t first, uint32_t bits,
-                                              uint32_t (&expert)[R], uint32_t (&rank)[R])
+__device__ __forceinline__ void load_experts(const OrderArgs& a, uint64_t first, uint32_t (&expert)[R])
 {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint64_t mine = first + wave * (64u * R) + lane;
+    const uint64_t mine = first + (threadIdx.x >> 6) * (64u * R) + (threadIdx.x & 63u);
 #pragma unroll
     for (uint32_t i = 0; i < R; ++i) {
         const uint64_t slot = mine + i * 64u;
         expert[i] = slot < a.slots ? static_cast<uint32_t>(a.ids[slot]) : a.experts;
     }
-    volatile uint16_t* count = sh.wave_count[wave];
+#pragma unroll
+    for (uint32_t i = 0; i < R; ++i)
+        if (expert[i] > a.experts) expert[i] = a.experts;
+}
+
+// Ranks slots inside their wave's stretch, and leaves its counts in the wave's row of counters.  Only the wave itself touches that
+// row, and its LDS accesses stay in order: no barrier here.
+template <uint32_t R>
+__device__ __forceinline__ void rank_in_waves(const OrderArgs& a, OrderShared& sh, uint32_t bits, const uint32_t (&expert)[R],
+                                              uint32_t (&rank)[R])
+{
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t* words = reinterpret_cast<uint32_t*>(sh.wave_count[wave]);
+    for (uint32_t w = lane; w < (a.experts + 1) / 2; w += 64) words[w] = 0;
+    wave_lds_sync();
 #pragma unroll
     for (uint32_t i = 0; i < R; ++i) {
-        if (expert[i] > a.experts) expert[i] = a.experts;
         const uint64_t same = same_value(expert[i], bits);
         const uint32_t below = __popcll(same & ((1ull << lane) - 1ull));
         rank[i] = below;
-        if (expert[i] < a.experts) {
-            const uint32_t before = count[expert[i]];
-            rank[i] += before;
-            if (below == 0) count[expert[i]] = static_cast<uint16_t>(before + __popcll(same));
-        }
+        uint32_t before = 0;
+        if (expert[i] < a.experts) before = sh.wave_count[wave][expert[i]];
+        rank[i] += before;
+        wave_lds_sync();
+        if (expert[i] < a.experts && below == 0) sh.wave_count[wave][expert[i]] = static_cast<uint16_t>(before + __popcll(same));
+        wave_lds_sync();
     }
 }
 
@@ -135,22 +147,32 @@ __device__ __forceinline__ void write_rows(const OrderArgs& a, const OrderShared
     }
 }
 
-// Rows without a slot: what fills the segments up, and everything behind the last one.
-__device__ __forceinline__ void mark_empty_rows(const OrderArgs& a, uint32_t e, uint32_t begin, uint32_t end)
+// Rows without a slot: what fills the segments up, shared out by expert among `blocks` workgroups and inside one among
+// groups of lanes as wide as a segment can need, and everything behind the last segment.
+__device__ __forceinline__ void mark_empty_rows(const OrderArgs& a, const OrderShared& sh, uint32_t end, uint32_t block, uint32_t blocks)
 {
-    (void)e;
-    if (end > a.rows) end = a.rows;
-    for (uint32_t r = begin; r < end; ++r) a.slot_of_row[r] = -1;
+    if (a.align > 1) {
+        uint32_t lanes = 64;
+        while (lanes > 1 && lanes / 2 >= a.align - 1) lanes /= 2;
+        for (uint32_t e = block + threadIdx.x / lanes * blocks; e < a.experts; e += kThreads / lanes * blocks) {
+            const uint32_t last = sh.fill_end[e] < a.rows ? sh.fill_end[e] : a.rows;
+            for (uint32_t r = sh.fill[e] + threadIdx.x % lanes; r < last; r += lanes) a.slot_of_row[r] = -1;
+        }
+    }
+    for (uint64_t r = static_cast<uint64_t>(end) + static_cast<uint64_t>(block) * kThreads + threadIdx.x; r < a.rows;
+         r += static_cast<uint64_t>(blocks) * kThreads)
+        a.slot_of_row[r] = -1;
 }
 
+// R slots a thread, all in one workgroup.
+template <uint32_t R>
 __global__ __launch_bounds__(kThreads) void route_order_small_kernel(const OrderArgs a, uint32_t bits)
 {
     __shared__ OrderShared sh;
     const uint32_t tid = threadIdx.x;
-    for (uint32_t i = tid; i < kWaves * a.experts; i += kThreads) sh.wave_count[i / a.experts][i % a.experts] = 0;
-    __syncthreads();
-    uint32_t expert[kSmallR], rank[kSmallR];
-    rank_in_waves<kSmallR>(a, sh, 0, bits, expert, rank);
+    uint32_t expert[R], rank[R];
+    load_experts<R>(a, 0, expert);
+    rank_in_waves<R>(a, sh, bits, expert, rank);
     __syncthreads();
     uint32_t kept = 0;
     if (tid < a.experts) {
@@ -163,14 +185,15 @@ __global__ __launch_bounds__(kThreads) void route_order_small_kernel(const Order
     if (tid < a.experts) {
         sh.row[tid] = offset;
         sh.room[tid] = a.capacity;
+        sh.fill[tid] = offset + kept;
+        sh.fill_end[tid] = offset + padded;
         a.counts[tid] = static_cast<int32_t>(kept);
         a.offsets[tid] = static_cast<int32_t>(offset);
         if (tid == a.experts - 1) a.offsets[a.experts] = static_cast<int32_t>(end);
-        mark_empty_rows(a, tid, offset + kept, offset + padded);
     }
-    for (uint64_t r = static_cast<uint64_t>(end) + tid; r < a.rows; r += kThreads) a.slot_of_row[r] = -1;
     __syncthreads();
-    write_rows<kSmallR>(a, sh, 0, expert, rank);
+    write_rows<R>(a, sh, 0, expert, rank);
+    mark_empty_rows(a, sh, end, 0, 1);
 }
 
 // tile_counts[block][e] = slots of expert e in the block's stretch of `per_block` slots
@@ -197,6 +220,11 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
     __shared__ uint32_t before_me[kMaxExperts];
     __shared__ uint32_t of_all[kMaxExperts];
     const uint32_t tid = threadIdx.x;
+    const uint64_t first = blockIdx.x * per_block;
+    uint64_t last = first + per_block;
+    if (last > a.slots) last = a.slots;
+    uint32_t expert[kTileR], rank[kTileR];
+    load_experts<kTileR>(a, first, expert);  // on their way while the counts are added up
     if (tid < a.experts) {
         before_me[tid] = 0;
         of_all[tid] = 0;
@@ -209,7 +237,7 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
     if (group < groups) {
         const uint32_t e = (tid - group * quads) * 4;
         uint32_t before[4] = {0, 0, 0, 0}, all[4] = {0, 0, 0, 0};
-#pragma unroll 8
+#pragma unroll 2
         for (uint32_t t = group; t < gridDim.x; t += groups) {
             const uint4 c = *reinterpret_cast<const uint4*>(a.tile_counts + static_cast<uint64_t>(t) * stride + e);
             const uint32_t mask = t < blockIdx.x ? 0xFFFFFFFFu : 0u;
@@ -238,30 +266,24 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
     if (tid < a.experts) {
         sh.row[tid] = offset + taken;
         sh.room[tid] = a.capacity - taken;
+        sh.fill[tid] = offset + kept;
+        sh.fill_end[tid] = offset + padded;
         if (blockIdx.x == 0) {
             a.counts[tid] = static_cast<int32_t>(kept);
             a.offsets[tid] = static_cast<int32_t>(offset);
             if (tid == a.experts - 1) a.offsets[a.experts] = static_cast<int32_t>(end);
         }
-        if (tid % gridDim.x == blockIdx.x) mark_empty_rows(a, tid, offset + kept, offset + padded);
     }
-    for (uint64_t r = static_cast<uint64_t>(end) + static_cast<uint64_t>(blockIdx.x) * kThreads + tid; r < a.rows;
-         r += static_cast<uint64_t>(gridDim.x) * kThreads)
-        a.slot_of_row[r] = -1;
-
-    const uint64_t first = blockIdx.x * per_block;
-    uint64_t last = first + per_block;
-    if (last > a.slots) last = a.slots;
-    for (uint64_t at = first; at < last; at += kTileSlots) {
-        for (uint32_t i = tid; i < kWaves * a.experts; i += kThreads) sh.wave_count[i / a.experts][i % a.experts] = 0;
-        __syncthreads();
-        uint32_t expert[kTileR], rank[kTileR];
-        rank_in_waves<kTileR>(a, sh, at, bits, expert, rank);
+    for (uint64_t at = first;;) {
+        rank_in_waves<kTileR>(a, sh, bits, expert, rank);
         __syncthreads();
         uint32_t in_tile = 0;
         if (tid < a.experts) in_tile = scan_waves(sh, tid);
         __syncthreads();
         write_rows<kTileR>(a, sh, at, expert, rank);
+        at += kTileSlots;
+        if (at >= last) break;
+        load_experts<kTileR>(a, at, expert);
         __syncthreads();
         if (tid < a.experts) {
             const uint32_t room = sh.room[tid];
@@ -270,6 +292,7 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
             sh.room[tid] = room - took;
         }
     }
+    mark_empty_rows(a, sh, end, blockIdx.x, gridDim.x);
 }
 
 }  // namespace
@@ -279,7 +302,10 @@ int launch_route_order(const OrderArgs& a, hipStream_t s)
     uint32_t bits = 0;
     while ((a.experts >> bits) != 0) ++bits;  // the values 0 .. experts
     if (a.slots <= kSmallSlots) {
-        hipLaunchKernelGGL(route_order_small_kernel, dim3(1), dim3(kThreads), 0, s, a, bits);
+        if (a.slots <= kThreads)
+            hipLaunchKernelGGL(route_order_small_kernel<1>, dim3(1), dim3(kThreads), 0, s, a, bits);
+        else
+            hipLaunchKernelGGL(route_order_small_kernel<8>, dim3(1), dim3(kThreads), 0, s, a, bits);
         MRS_CHECK_LAUNCH("route_order_small_kernel");
         return MRS_OK;
     }

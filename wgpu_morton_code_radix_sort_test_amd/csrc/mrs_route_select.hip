@@ -1,11 +1,12 @@
 // The topk largest of every row of scores, the weights they give, and the scores' gradient
 // (mrs_route_select, mrs_route_select_backward in include/mrs.h).
 //
-// A row belongs to a group of L lanes, V elements a lane.  A key and its column travel together in the
-// 52 mantissa bits of a double in [1, 2) -- the key mapped to an unsigned number of the same order in
-// the upper 32, the complement of the column below -- so that one 64-bit maximum picks the larger key and, of
-// equal keys, the lower column.  Every lane sorts its V elements once; a step takes the largest
-// head of the group's lists.
+// A row belongs to a group of L lanes, V columns a lane in runs of up to 16 bytes.  A key and its column travel together
+// in the 52 mantissa bits of a double in [1, 2) -- the key mapped to an unsigned number of the same order in the upper
+// 32, the complement of the column below -- so that one 64-bit maximum picks the larger key and, of equal keys, the
+// lower column.  Every lane sorts its V columns once by a network of such maxima and minima; a step then takes the largest head
+// of the group's lists, found by rotations inside a row of 16 lanes.  For few slots the steps are unrolled, and only
+// as much of a list is kept and moved up as later steps can ask for.
 #include "mrs_route.hpp"
 
 namespace mrs {
@@ -14,8 +15,9 @@ namespace {
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMaxBlocks = 1u << 20;
-constexpr uint32_t kColumnMask = 0x3FFu;  // MRS_ROUTE_MAX_EXPERTS - 1
+constexpr uint32_t kColumnMask = 0x3FFu;      // MRS_ROUTE_MAX_EXPERTS - 1
 constexpr uint32_t kLowestKey = 0x007FFFFFu;  // -infinity; keys that take part are above
+constexpr float kLog2E = 1.44269504088896340736f;
 static_assert(MRS_ROUTE_MAX_EXPERTS <= kColumnMask + 1, "a column fits its bits");
 
 // The order of floats as an order of unsigned numbers; 0 for what does not take part.
@@ -36,26 +38,55 @@ __device__ __forceinline__ uint32_t packed_column(double p)
     return kColumnMask - (static_cast<uint32_t>(__builtin_bit_cast(uint64_t, p)) & kColumnMask);
 }
 
-template <uint32_t L>
-__device__ __forceinline__ double group_max(double v)
+// The value M lanes on: inside a row of 16 lanes by a rotation, which after steps of 8, 4, 2 and 1 has combined all of them like an
+// exchange does; across rows by an exchange.
+template <uint32_t M>
+__device__ __forceinline__ uint32_t neighbour(uint32_t v)
 {
-#pragma unroll
-    for (uint32_t m = L / 2; m > 0; m /= 2) v = fmax(v, __shfl_xor(v, static_cast<int>(m), static_cast<int>(L)));
-    return v;
+    if constexpr (M < 16)
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x120 + M, 0xF, 0xF, false));  // row_ror
+    else if constexpr (M == 16)
+        return static_cast<uint32_t>(__builtin_amdgcn_ds_swizzle(static_cast<int>(v), 0x401F));  // lane ^ 16
+    else
+        return __shfl_xor(v, static_cast<int>(M));
 }
-template <uint32_t L>
-__device__ __forceinline__ float group_max(float v)
+template <uint32_t M>
+__device__ __forceinline__ float neighbour(float v)
 {
-#pragma unroll
-    for (uint32_t m = L / 2; m > 0; m /= 2) v = fmaxf(v, __shfl_xor(v, static_cast<int>(m), static_cast<int>(L)));
-    return v;
+    return __builtin_bit_cast(float, neighbour<M>(__builtin_bit_cast(uint32_t, v)));
 }
-template <uint32_t L>
-__device__ __forceinline__ float group_sum(float v)
+template <uint32_t M>
+__device__ __forceinline__ double neighbour(double v)
 {
-#pragma unroll
-    for (uint32_t m = L / 2; m > 0; m /= 2) v += __shfl_xor(v, static_cast<int>(m), static_cast<int>(L));
-    return v;
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint64_t low = neighbour<M>(static_cast<uint32_t>(bits)), high = neighbour<M>(static_cast<uint32_t>(bits >> 32));
+    return __builtin_bit_cast(double, low | high << 32);
+}
+template <uint32_t M>
+__device__ __forceinline__ double max_of_group(double v)
+{
+    if constexpr (M == 0)
+        return v;
+    else
+        return max_of_group<M / 2>(fmax(v, neighbour<M>(v)));
+}
+template <uint32_t M>
+__device__ __forceinline__ float max_of_group(float v)
+{
+    if constexpr (M == 0)
+        return v;
+    else
+        return max_of_group<M / 2>(fmaxf(v, neighbour<M>(v)));
+}
+// Every lane adds the same numbers, in an order of its own inside a row of 16; what matters is that it is fixed.  The first
+// lane's sum is given to all.
+template <uint32_t M>
+__device__ __forceinline__ float add_group(float v)
+{
+    if constexpr (M == 0)
+        return v;
+    else
+        return add_group<M / 2>(v + neighbour<M>(v));
 }
 
 // log(1 / (1 + exp(-s))), without overflow on either side
@@ -66,58 +97,119 @@ __device__ __forceinline__ float sigmoid(float s)
     return (s >= 0.0f ? 1.0f : x) / (1.0f + x);
 }
 
-// Maximum and sum of exponentials of the row's scores that take part.  NaN if one is +infinity.
+// How a group of L lanes shares a row: V columns a lane, in runs of W.
 template <typename T, uint32_t L, uint32_t V>
-__device__ __forceinline__ void softmax_of_row(const float (&s)[V], const bool (&part)[V], float* m, float* sum)
+struct Share {
+    static constexpr uint32_t W = V * sizeof(T) < 16 ? V : 16 / sizeof(T);
+    static_assert(V % W == 0);
+    struct __attribute__((packed, aligned(sizeof(T)))) Run {
+        T e[W];
+    };
+    __device__ static uint32_t column(uint32_t lane, uint32_t i) { return (i / W * L + lane) * W + i % W; }
+
+    // -infinity behind the last column
+    __device__ static void load(const T* row, uint32_t experts, uint32_t lane, float (&s)[V])
+    {
+#pragma unroll
+        for (uint32_t c = 0; c < V / W; ++c) {
+            const uint32_t e = (c * L + lane) * W;
+            if (e + W <= experts) {
+                const Run run = *reinterpret_cast<const Run*>(row + e);
+#pragma unroll
+                for (uint32_t i = 0; i < W; ++i) s[c * W + i] = to_f32(run.e[i]);
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < W; ++i) s[c * W + i] = e + i < experts ? to_f32(row[e + i]) : -__builtin_inff();
+            }
+        }
+    }
+    __device__ static void store(T* row, uint32_t experts, uint32_t lane, const float (&s)[V])
+    {
+#pragma unroll
+        for (uint32_t c = 0; c < V / W; ++c) {
+            const uint32_t e = (c * L + lane) * W;
+            if (e + W <= experts) {
+                Run run;
+#pragma unroll
+                for (uint32_t i = 0; i < W; ++i) run.e[i] = static_cast<T>(s[c * W + i]);
+                *reinterpret_cast<Run*>(row + e) = run;
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < W; ++i)
+                    if (e + i < experts) row[e + i] = static_cast<T>(s[c * W + i]);
+            }
+        }
+    }
+    // the keys choices are made by
+    __device__ static void keys(const float* __restrict__ bias, uint32_t experts, uint32_t lane, const float (&s)[V], float (&key)[V])
+    {
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) key[i] = s[i];
+        if (!bias) return;
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) key[i] += bias[min(column(lane, i), experts - 1)];
+    }
+};
+
+// Maximum m of the row's scores that take part and sum of exp(s - m); the others become -infinity, whose exponential is 0
+// (a row of them: NaN that nobody reads).  exp(s - m) is 2^(s log2 e - m log2 e), off by 2 |s - m| + 2 roundings at most.
+template <uint32_t L, uint32_t V>
+__device__ __forceinline__ void softmax_of_row(float (&s)[V], const float (&key)[V], float* m, float* sum)
 {
     float top = -__builtin_inff();
 #pragma unroll
-    for (uint32_t i = 0; i < V; ++i)
-        if (part[i]) top = fmaxf(top, s[i]);
-    *m = group_max<L>(top);
+    for (uint32_t i = 0; i < V; ++i) {
+        if (!(key[i] > -__builtin_inff())) s[i] = -__builtin_inff();
+        top = fmaxf(top, s[i]);
+    }
+    *m = max_of_group<L / 2>(top);
     float total = 0.0f;
 #pragma unroll
-    for (uint32_t i = 0; i < V; ++i)
-        if (part[i]) total += expf(s[i] - *m);
-    *sum = group_sum<L>(total);
+    for (uint32_t i = 0; i < V; ++i) total += __builtin_amdgcn_exp2f((s[i] - *m) * kLog2E);
+    *sum = __shfl(add_group<L / 2>(total), 0, static_cast<int>(L));
 }
 
-// The row's scores, and which of them take part.  Lane l holds the columns i * L + l.
-template <typename T, uint32_t L, uint32_t V>
-__device__ __forceinline__ void load_row(const SelectArgs& a, uint64_t t, uint32_t lane, float (&s)[V], float (&key)[V])
+// Step J of the unrolled form: lane J keeps the largest head, and the list it came from moves up -- as far as the steps
+// still to come can reach.
+template <uint32_t L, uint32_t J, uint32_t D>
+__device__ __forceinline__ void take_largest(double (&list)[D], uint32_t topk, uint32_t lane, double* mine)
 {
-    const T* row = static_cast<const T*>(a.scores) + t * a.ld_scores;
+    constexpr uint32_t kSteps = 8;
+    if constexpr (J < kSteps) {
+        if (J >= topk) return;
+        const double top = max_of_group<L / 2>(list[0]);
+        if (lane == J) *mine = top;
+        const bool taken = list[0] == top;
+        constexpr uint32_t kLeft = kSteps - 1 - J < D ? kSteps - 1 - J : D;
 #pragma unroll
-    for (uint32_t i = 0; i < V; ++i) {
-        const uint32_t e = i * L + lane;
-        s[i] = -__builtin_inff();
-        key[i] = -__builtin_inff();
-        if (e < a.experts) {
-            s[i] = to_f32(row[e]);
-            key[i] = a.bias ? s[i] + a.bias[e] : s[i];
+        for (uint32_t i = 0; i < kLeft; ++i) {
+            if constexpr (D > 1)
+                list[i] = taken ? (i + 1 < D ? list[i + 1 < D ? i + 1 : i] : 1.0) : list[i];
+            else
+                list[i] = taken ? 1.0 : list[i];
         }
+        take_largest<L, J + 1, D>(list, topk, lane, mine);
     }
 }
 
-template <typename T, uint32_t L, uint32_t V>
-__global__ __launch_bounds__(kThreads) void route_select_kernel(const SelectArgs a)
+template <typename T, uint32_t L, uint32_t V, bool FEW>
+__global__ __launch_bounds__(kThreads) void route_select_kernel(const T* __restrict__ scores, const float* __restrict__ bias,
+                                                                const SelectArgs a)
 {
+    using S = Share<T, L, V>;
     constexpr uint32_t kGroups = kThreads / L;
     const uint32_t lane = threadIdx.x & (L - 1);
     for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kGroups + threadIdx.x / L; t < a.tokens;
          t += static_cast<uint64_t>(gridDim.x) * kGroups) {
+        const T* row = scores + t * a.ld_scores;
         float s[V], key[V];
-        load_row<T, L, V>(a, t, lane, s, key);
-        float m = 0.0f, sum = 1.0f;
-        if (a.gate == MRS_GATE_SOFTMAX && !a.normalize) {
-            bool part[V];
-#pragma unroll
-            for (uint32_t i = 0; i < V; ++i) part[i] = key[i] > -__builtin_inff();
-            softmax_of_row<T, L, V>(s, part, &m, &sum);
-        }
+        S::load(row, a.experts, lane, s);
+        S::keys(bias, a.experts, lane, s, key);
         double list[V];
 #pragma unroll
-        for (uint32_t i = 0; i < V; ++i) list[i] = pack(ordered_key(key[i]), i * L + lane);
+        for (uint32_t i = 0; i < V; ++i) list[i] = pack(ordered_key(key[i]), S::column(lane, i));
+        float m = 0.0f, sum = 1.0f;
+        if (a.gate == MRS_GATE_SOFTMAX && !a.normalize) softmax_of_row<L, V>(s, key, &m, &sum);
         // odd-even merge sort, largest first
 #pragma unroll
         for (uint32_t p = 1; p < V; p *= 2)
@@ -128,32 +220,40 @@ __global__ __launch_bounds__(kThreads) void route_select_kernel(const SelectArgs
 #pragma unroll
                     for (uint32_t i = 0; i < k; ++i)
                         if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
-                            const double hi = fmax(list[i + j], list[i + j + k]);
-                            const double lo = fmin(list[i + j], list[i + j + k]);
-                            list[i + j] = hi;
-                            list[i + j + k] = lo;
+                            const double high = fmax(list[i + j], list[i + j + k]);
+                            const double low = fmin(list[i + j], list[i + j + k]);
+                            list[i + j] = high;
+                            list[i + j + k] = low;
                         }
         double mine = 1.0;  // lane j keeps the j-th largest
-        for (uint32_t j = 0; j < a.topk; ++j) {
-            const double top = group_max<L>(list[0]);
-            if (lane == j) mine = top;
-            if (list[0] == top) {
+        if constexpr (FEW) {
+            constexpr uint32_t kDepth = V < 8 ? V : 8;
+            double heads[kDepth];
 #pragma unroll
-                for (uint32_t i = 0; i + 1 < V; ++i) list[i] = list[i + 1];
-                list[V - 1] = 1.0;
+            for (uint32_t i = 0; i < kDepth; ++i) heads[i] = list[i];
+            take_largest<L, 0, kDepth>(heads, a.topk, lane, &mine);
+        } else {
+            for (uint32_t j = 0; j < a.topk; ++j) {
+                const double top = max_of_group<L / 2>(list[0]);
+                if (lane == j) mine = top;
+                if (list[0] == top) {
+#pragma unroll
+                    for (uint32_t i = 0; i + 1 < V; ++i) list[i] = list[i + 1];
+                    list[V - 1] = 1.0;
+                }
             }
         }
         const bool used = lane < a.topk;
         const bool chosen = used && packed_key(mine) > kLowestKey;
         const uint32_t e = packed_column(mine);
-        float w = 0.0f;
-        const float score = chosen ? to_f32(static_cast<const T*>(a.scores)[t * a.ld_scores + e]) : -__builtin_inff();
+        const float score = chosen ? to_f32(row[e]) : -__builtin_inff();
+        float w;
         if (a.normalize) {
             // p[id] / sum of p over the slots, as a softmax over the slots of log p
             const float x = a.gate == MRS_GATE_SOFTMAX ? score : chosen ? log_sigmoid(score) : score;
-            const float top = group_max<L>(x);
+            const float top = max_of_group<L / 2>(x);
             w = chosen ? expf(x - top) : 0.0f;
-            w = w / group_sum<L>(w);
+            w = w / __shfl(add_group<L / 2>(w), 0, static_cast<int>(L));
         } else if (a.gate == MRS_GATE_SOFTMAX) {
             w = expf(score - m) / sum;
         } else {
@@ -166,71 +266,82 @@ __global__ __launch_bounds__(kThreads) void route_select_kernel(const SelectArgs
     }
 }
 
-// The gradient: the slots' derivatives are worked out by the first lanes of the group, laid into a row in LDS and
-// written out with the rest of the row.
+// The gradient.  The slots' derivatives are worked out by the first lanes of the group and laid into a row in LDS, which is written
+// out, less p[e] times their sum where the softmax runs over the whole row.
 template <typename T, uint32_t L, uint32_t V>
-__global__ __launch_bounds__(kThreads) void route_select_backward_kernel(const SelectArgs a)
+__global__ __launch_bounds__(kThreads) void route_select_backward_kernel(const T* __restrict__ scores, const float* __restrict__ bias,
+                                                                         T* __restrict__ scores_grad, const SelectArgs a)
 {
+    using S = Share<T, L, V>;
     constexpr uint32_t kGroups = kThreads / L;
     __shared__ float grads[kGroups][L * V];
-    const uint32_t lane = threadIdx.x & (L - 1);
-    volatile float* grad = grads[threadIdx.x / L];
+    const uint32_t lane = threadIdx.x & (L - 1), group = threadIdx.x / L;
     const bool whole_row = a.gate == MRS_GATE_SOFTMAX && !a.normalize;
-    for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kGroups + threadIdx.x / L; t < a.tokens;
+    for (uint64_t t = static_cast<uint64_t>(blockIdx.x) * kGroups + group; t < a.tokens;
          t += static_cast<uint64_t>(gridDim.x) * kGroups) {
-        float s[V], key[V];
-        float m = 0.0f, sum = 1.0f;
-        bool part[V];
-        if (whole_row) {
-            load_row<T, L, V>(a, t, lane, s, key);
-#pragma unroll
-            for (uint32_t i = 0; i < V; ++i) part[i] = key[i] > -__builtin_inff();
-            softmax_of_row<T, L, V>(s, part, &m, &sum);
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < V; ++i) grad[i * L + lane] = 0.0f;
+        const T* row = scores + t * a.ld_scores;
         const bool used = lane < a.topk;
         const uint32_t id = used ? static_cast<uint32_t>(a.ids[t * a.topk + lane]) : 0xFFFFFFFFu;
+        const float dw = used ? a.weights_grad[t * a.topk + lane] : 0.0f;
+        float m = 0.0f, sum = 1.0f;
+        float s[V];
+        if (whole_row) {
+            float key[V];
+            S::load(row, a.experts, lane, s);
+            S::keys(bias, a.experts, lane, s, key);
+            softmax_of_row<L, V>(s, key, &m, &sum);
+        }
         float score = -__builtin_inff();
         bool chosen = id < a.experts;
         if (chosen) {
-            score = to_f32(static_cast<const T*>(a.scores)[t * a.ld_scores + id]);
-            chosen = (a.bias ? score + a.bias[id] : score) > -__builtin_inff();
+            score = to_f32(row[id]);
+            chosen = (bias ? score + bias[id] : score) > -__builtin_inff();
         }
-        const float g = chosen ? a.weights_grad[t * a.topk + lane] * a.scale : 0.0f;
+        const float g = chosen ? dw * a.scale : 0.0f;
         float d;
         float all = 0.0f;
         if (a.normalize) {
             const float x = !chosen ? -__builtin_inff() : a.gate == MRS_GATE_SOFTMAX ? score : log_sigmoid(score);
-            const float top = group_max<L>(x);
+            const float top = max_of_group<L / 2>(x);
             float q = chosen ? expf(x - top) : 0.0f;
-            q = q / group_sum<L>(q);
-            const float mean = group_sum<L>(chosen ? q * g : 0.0f);
+            q = q / __shfl(add_group<L / 2>(q), 0, static_cast<int>(L));
+            const float mean = __shfl(add_group<L / 2>(chosen ? q * g : 0.0f), 0, static_cast<int>(L));
             d = q * (g - mean);
             if (a.gate == MRS_GATE_SIGMOID) d *= sigmoid(-score);
         } else if (a.gate == MRS_GATE_SOFTMAX) {
             d = expf(score - m) / sum * g;
-            all = group_sum<L>(chosen ? d : 0.0f);
+            all = __shfl(add_group<L / 2>(chosen ? d : 0.0f), 0, static_cast<int>(L));
         } else {
             d = sigmoid(score) * sigmoid(-score) * g;
         }
-        // a repeated id: all its slots hold the sum, added in the order of the slots
-        float total = 0.0f;
-        for (uint32_t j = 0; j < a.topk; ++j) {
-            const uint32_t other = __shfl(id, static_cast<int>(j), static_cast<int>(L));
-            const float x = __shfl(d, static_cast<int>(j), static_cast<int>(L));
-            if (other == id) total += x;
-        }
-        if (chosen) grad[id] = total;
-        T* out = static_cast<T*>(a.scores_grad) + t * a.ld_scores_grad;
+        // ids that repeat show by a lane not finding its own mark; their slots are then added one after the other
+        if (chosen) grads[group][id] = static_cast<float>(lane);
+        wave_lds_sync();
+        const bool repeated = chosen && grads[group][id] != static_cast<float>(lane);
+        wave_lds_sync();
 #pragma unroll
-        for (uint32_t i = 0; i < V; ++i) {
-            const uint32_t e = i * L + lane;
-            if (e >= a.experts) continue;
-            float x = grad[e];
-            if (whole_row && part[i]) x -= expf(s[i] - m) / sum * all;
-            out[e] = static_cast<T>(x);
+        for (uint32_t i = 0; i < V; ++i) grads[group][i * L + lane] = 0.0f;
+        wave_lds_sync();
+        if (__ballot(repeated)) {
+            for (uint32_t j = 0; j < a.topk; ++j) {
+                if (lane == j && chosen) grads[group][id] = grads[group][id] + d;
+                wave_lds_sync();
+            }
+        } else if (chosen) {
+            grads[group][id] = d;
         }
+        wave_lds_sync();
+        const float share = all / sum;
+        float out[V];
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) out[i] = grads[group][S::column(lane, i)];
+        wave_lds_sync();
+        if (whole_row) {
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i)
+                if (s[i] > -__builtin_inff()) out[i] -= __builtin_amdgcn_exp2f((s[i] - m) * kLog2E) * share;
+        }
+        S::store(scores_grad + t * a.ld_scores_grad, a.experts, lane, out);
     }
 }
 
@@ -241,10 +352,13 @@ void start(const SelectArgs& a, bool backward, hipStream_t s)
     uint64_t blocks = (a.tokens + kGroups - 1) / kGroups;
     if (blocks > kMaxBlocks) blocks = kMaxBlocks;
     const dim3 grid(static_cast<uint32_t>(blocks)), block(kThreads);
+    const T* scores = static_cast<const T*>(a.scores);
     if (backward)
-        hipLaunchKernelGGL((route_select_backward_kernel<T, L, V>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((route_select_backward_kernel<T, L, V>), grid, block, 0, s, scores, a.bias, static_cast<T*>(a.scores_grad), a);
+    else if (a.topk <= 8)
+        hipLaunchKernelGGL((route_select_kernel<T, L, V, true>), grid, block, 0, s, scores, a.bias, a);
     else
-        hipLaunchKernelGGL((route_select_kernel<T, L, V>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((route_select_kernel<T, L, V, false>), grid, block, 0, s, scores, a.bias, a);
 }
 
 // Lanes of a row: 16, more where topk (a slot per lane at the end) or 16 columns a lane ask for it.
@@ -260,8 +374,6 @@ void choose(const SelectArgs& a, bool backward, hipStream_t s)
             start<T, 16, 8>(a, backward, s);
         else
             start<T, 16, 16>(a, backward, s);
-    } else if (a.experts <= 128) {
-        start<T, 32, 4>(a, backward, s);
     } else if (a.experts <= 512) {
         start<T, 32, 16>(a, backward, s);
     } else {
