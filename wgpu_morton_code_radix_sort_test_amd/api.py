@@ -490,19 +490,19 @@ class RoutePlan:
             raise ValueError(f"{name} must have two dimensions, not {t.dim()}")
         return t.size(0)
 
-    def _indices(self, t, name, least):
-        if t.device != self.device:
-            self._on_device(t, name)
-        if t.dtype != torch.int32 or t.numel() < least or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 tensor of at least {least} elements")
-        return t.data_ptr()
-
     def _map(self, route, tokens):
-        return _lib.RouteMapStruct(self._indices(route.row_of_slot, "row_of_slot", tokens * self.topk),
-                                   self._indices(route.slot_of_row, "slot_of_row", 0),
-                                   self._indices(route.counts, "counts", self.experts),
-                                   self._indices(route.offsets, "offsets", self.experts + 1),
-                                   route.slot_of_row.numel()), route.slot_of_row.numel()
+        """The map's structure for the library, and its number of rows."""
+        device, int32 = self.device, torch.int32
+        to_row, to_slot, counts, offsets = route.row_of_slot, route.slot_of_row, route.counts, route.offsets
+        if not (to_row.device == to_slot.device == counts.device == offsets.device == device):
+            raise ValueError(f"a tensor of the map is on another device than the plan, which is on {device}")
+        if not (to_row.dtype is int32 and to_slot.dtype is int32 and counts.dtype is int32 and offsets.dtype is int32
+                and to_row.is_contiguous() and to_slot.is_contiguous() and counts.is_contiguous() and offsets.is_contiguous()):
+            raise ValueError("the tensors of the map must be contiguous and int32")
+        if to_row.numel() < tokens * self.topk or counts.numel() < self.experts or offsets.numel() <= self.experts:
+            raise ValueError(f"the map is too small for {tokens} tokens, {self.topk} slots each, and {self.experts} experts")
+        rows = to_slot.numel()
+        return _lib.RouteMapStruct(to_row.data_ptr(), to_slot.data_ptr(), counts.data_ptr(), offsets.data_ptr(), rows), rows
 
     def _on_stream(self, stream):
         return _raw_stream(self.device.index) if stream is None else stream.cuda_stream

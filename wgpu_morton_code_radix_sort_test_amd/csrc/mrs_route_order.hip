@@ -7,10 +7,11 @@
 // the equal lanes below; a scan over the waves' counters gives the rank inside the tile.  No
 // atomics decide an order, so rows are the same every time.
 //
-// Up to kSmallSlots slots one workgroup does everything in one launch; what bounds it is the chain of
-// LDS accesses and barriers.  Above, a first launch counts tiles, and in a second one
-// every workgroup adds up the counts of the tiles before its own by itself (at most 256 tiles of
-// `experts` counts, read from L2) instead of waiting for a scan launch between the two.
+// Up to kSmallSlots slots one workgroup does everything in one launch (512 slots, 256 experts: 4.0 us); what bounds it is
+// the launch and the chain of LDS accesses and barriers.  Above, a first launch counts tiles, and in a second one every
+// workgroup adds up the counts of the tiles before its own by itself (at most 256 tiles of `experts` counts, read from
+// L2) instead of waiting for a scan launch between the two.  2^20 slots, 256 experts: 17 us, 4 of them for the counts, about 3 each for
+// adding them up and for the writes to slot_of_row in runs of some 16 rows.
 #include "mrs_route.hpp"
 
 namespace mrs {
@@ -224,25 +225,39 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
     uint64_t last = first + per_block;
     if (last > a.slots) last = a.slots;
     uint32_t expert[kTileR], rank[kTileR];
-    load_experts<kTileR>(a, first, expert);  // on their way while the counts are added up
+    load_experts<kTileR>(a, first, expert);
     if (tid < a.experts) {
         before_me[tid] = 0;
         of_all[tid] = 0;
     }
+    rank_in_waves<kTileR>(a, sh, bits, expert, rank);
     __syncthreads();
-    // the counts of all tiles, four experts a thread, the tiles shared out among groups of threads
+    // The counts of all tiles, four experts a thread, the tiles shared out among groups of threads.  Every workgroup begins
+    // with its own: all of them reading the same tile at a time took 3 us longer.  Four loads at a time; a thread that has fewer
+    // tiles left reads one again.
     const uint32_t quads = stride / 4;
     const uint32_t groups = kThreads / quads;
     const uint32_t group = tid / quads;
     if (group < groups) {
         const uint32_t e = (tid - group * quads) * 4;
         uint32_t before[4] = {0, 0, 0, 0}, all[4] = {0, 0, 0, 0};
-#pragma unroll 2
-        for (uint32_t t = group; t < gridDim.x; t += groups) {
-            const uint4 c = *reinterpret_cast<const uint4*>(a.tile_counts + static_cast<uint64_t>(t) * stride + e);
-            const uint32_t mask = t < blockIdx.x ? 0xFFFFFFFFu : 0u;
-            all[0] += c.x, all[1] += c.y, all[2] += c.z, all[3] += c.w;
-            before[0] += c.x & mask, before[1] += c.y & mask, before[2] += c.z & mask, before[3] += c.w & mask;
+        for (uint32_t i0 = group; i0 < gridDim.x; i0 += 4 * groups) {
+            uint4 c[4];
+            uint32_t t[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                const uint32_t i = i0 + k * groups;
+                t[k] = (i < gridDim.x ? i : i0) + blockIdx.x;
+                if (t[k] >= gridDim.x) t[k] -= gridDim.x;
+                c[k] = *reinterpret_cast<const uint4*>(a.tile_counts + static_cast<uint64_t>(t[k]) * stride + e);
+                if (i >= gridDim.x) c[k] = make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                const uint32_t mask = t[k] < blockIdx.x ? 0xFFFFFFFFu : 0u;
+                all[0] += c[k].x, all[1] += c[k].y, all[2] += c[k].z, all[3] += c[k].w;
+                before[0] += c[k].x & mask, before[1] += c[k].y & mask, before[2] += c[k].z & mask, before[3] += c[k].w & mask;
+            }
         }
         // whole numbers: the order of these additions does not matter
 #pragma unroll
@@ -253,8 +268,9 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
             }
     }
     __syncthreads();
-    uint32_t kept = 0, taken = 0;
+    uint32_t kept = 0, taken = 0, in_tile = 0;
     if (tid < a.experts) {
+        in_tile = scan_waves(sh, tid);
         kept = of_all[tid];
         if (kept > a.capacity) kept = a.capacity;
         taken = before_me[tid];
@@ -274,12 +290,8 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
             if (tid == a.experts - 1) a.offsets[a.experts] = static_cast<int32_t>(end);
         }
     }
+    __syncthreads();
     for (uint64_t at = first;;) {
-        rank_in_waves<kTileR>(a, sh, bits, expert, rank);
-        __syncthreads();
-        uint32_t in_tile = 0;
-        if (tid < a.experts) in_tile = scan_waves(sh, tid);
-        __syncthreads();
         write_rows<kTileR>(a, sh, at, expert, rank);
         at += kTileSlots;
         if (at >= last) break;
@@ -291,6 +303,10 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
             sh.row[tid] += took;
             sh.room[tid] = room - took;
         }
+        rank_in_waves<kTileR>(a, sh, bits, expert, rank);
+        __syncthreads();
+        if (tid < a.experts) in_tile = scan_waves(sh, tid);
+        __syncthreads();
     }
     mark_empty_rows(a, sh, end, blockIdx.x, gridDim.x);
 }
