@@ -136,7 +136,7 @@ int mrs_context_destroy(mrs_context* ctx);
  * librocprofiler-sdk-roctx.so or libroctx64.so) named as the reference names the pass it stands
  * for: "Morton Coding", "Histogram calculation", "Large Prefix Sum part 1", "Small Prefix Sum",
  * "Large Prefix Sum part 2", "Indexing"; launches without a counterpart there are named for what
- * they do ("Clear", "Local sort", "Gather").  `rocprofv3 --marker-trace --kernel-trace` then reads
+ * they do ("Clear", "Local sort", "Gather", "Select", "Order", "Dispatch", "Combine").  `rocprofv3 --marker-trace --kernel-trace` then reads
  * like the reference's NSight capture.  Setting it fails with MRS_ERR_UNSUPPORTED if no roctx
  * library can be loaded. */
 #define MRS_ATTR_ROCTX_RANGES 4
@@ -527,7 +527,8 @@ int mrs_splitter_get(const mrs_splitter* sp, mrs_split_result* out);
  * kernels on `stream` (no allocation, no memset, no synchronisation) and may be captured into a HIP
  * graph; results do not depend on timing (no floating-point atomics).  Only mrs_route_order uses
  * memory of the handle: calls of it on one handle, and replays of graphs that hold one, must not
- * overlap in time.  Buffers need the alignment of their element, nothing more. */
+ * overlap in time, and the handle has to outlive such graphs.  Buffers need the alignment of their
+ * element, nothing more; no output may overlap an input or another output. */
 typedef struct mrs_route mrs_route;
 
 #define MRS_GATE_SOFTMAX 0 /* p[e] = exp(s[e]) / sum of exp(s) over the experts that take part      */
@@ -578,8 +579,7 @@ int mrs_route_select(mrs_route* route, uint64_t tokens, const void* scores_dev, 
                      const float* bias_dev, int32_t* ids_dev, float* weights_dev, void* stream);
 /* scores_grad[t, e] = sum over j of weights_grad[t, j] * d weights[t, j] / d scores[t, e] for the ids
  * given (mrs_route_select's; ids that are negative, too large or masked count for nothing; a repeated
- * id is as many slots).  All `experts` elements of each row are written.  scores_grad must not overlap
- * the inputs. */
+ * id is as many slots).  All `experts` elements of each row are written. */
 int mrs_route_select_backward(mrs_route* route, uint64_t tokens, const void* scores_dev, uint64_t ld_scores, int32_t type,
                               const float* bias_dev, const int32_t* ids_dev, const float* weights_grad_dev,
                               void* scores_grad_dev, uint64_t ld_scores_grad, void* stream);
@@ -589,7 +589,7 @@ int mrs_route_order(mrs_route* route, uint64_t tokens, const int32_t* ids_dev, c
 /* rows[row_of_slot[t, j]] = x[t]; rows of a segment that no slot has (they fill it up to `align`) are
  * zeroed, rows from offsets[experts] on are left as they are.  Indices outside [0, map->rows) are
  * passed over, here and below.  x: `tokens` rows ld_x elements apart; rows: map->rows rows ld_rows
- * apart; the two must not overlap. */
+ * apart. */
 int mrs_route_dispatch(mrs_route* route, uint64_t tokens, const mrs_route_map* map, int32_t type, uint64_t hidden,
                        const void* x_dev, uint64_t ld_x, void* rows_dev, uint64_t ld_rows, void* stream);
 /* x_grad[t] = sum over j of rows_grad[row_of_slot[t, j]], in 32 bits in the order of j, rounded once;
@@ -604,7 +604,7 @@ int mrs_route_combine(mrs_route* route, uint64_t tokens, const mrs_route_map* ma
                       void* stream);
 /* rows_grad[row_of_slot[t, j]] = weights[t, j] * out_grad[t] (rounded once; other rows as in
  * mrs_route_dispatch) and weights_grad[t, j] = sum over h of out_grad[t, h] * rows[row_of_slot[t, j], h] in
- * 32 bits, 0 for a slot without a row.  rows_grad must not overlap the inputs. */
+ * 32 bits, 0 for a slot without a row. */
 int mrs_route_combine_backward(mrs_route* route, uint64_t tokens, const mrs_route_map* map, int32_t type, uint64_t hidden,
                                const void* out_grad_dev, uint64_t ld_out_grad, const void* rows_dev, uint64_t ld_rows,
                                const float* weights_dev, void* rows_grad_dev, uint64_t ld_rows_grad, float* weights_grad_dev,

@@ -80,7 +80,8 @@ def check_select(mrs, ctx, scores, bias, topk, gate, normalize, scale, strided=F
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("tokens,experts,topk", [(1, 1, 1), (1, 8, 2), (3, 7, 7), (5, 16, 16), (17, 60, 6), (33, 64, 8),
                                                  (2, 33, 32), (40, 128, 8), (9, 129, 10), (70, 256, 8), (3, 257, 16), (4, 512, 32),
-                                                 (2, 1000, 22), (3, 1024, 32)])
+                                                 (2, 1000, 22), (3, 1024, 32), (6, 300, 4), (5, 512, 8),
+                                                 (4, 513, 3), (3, 1024, 8), (7, 600, 1), (9, 33, 9)])
 def test_select(ctx, mrs, tokens, experts, topk, dtype, gate, normalize):
     g = torch.Generator().manual_seed(tokens * 1000 + experts)
     scores = (torch.randn(tokens, experts, generator=g) * 2).to(dtype)  # 16-bit scores hold many equal ones
@@ -521,6 +522,39 @@ def test_calls_take_the_stream_they_are_given(ctx, mrs):
         assert torch.equal(getattr(route, name), getattr(want, name))
 
 
+def test_new_outputs_belong_to_the_stream_that_writes_them(ctx, mrs):
+    """Memory just freed on the current stream, where work that writes it is still queued, must not become the output of a call on
+    another stream: the queued work would overwrite it afterwards."""
+    dev = ctx.device
+    plan = mrs.RoutePlan(ctx, 4096, 8, 1)
+    ids = torch.zeros(4096, 1, dtype=torch.int32, device=dev)
+    route, w = plan.order(ids), torch.ones(4096, 1, device=dev)
+    rows = torch.ones(4096, 512, device=dev)
+    other = torch.cuda.Stream()
+    big = torch.randn(8192, 8192, device=dev)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    scrap = torch.empty(4096, 512, device=dev)
+    place = scrap.data_ptr()
+    for _ in range(10):
+        big = big @ big * 1e-3
+    scrap.fill_(7.0)
+    del scrap
+    out = plan.combine(rows, route, w, stream=other)
+    other.synchronize()
+    torch.cuda.synchronize()
+    assert out.data_ptr() != place and bool((out == 1).all())
+
+
+def test_eight_bit_floats_are_moved_unseen(ctx, mrs):
+    plan, route, rows, g = make_route(mrs, ctx, 40, 8, 2, 4)
+    x = torch.randint(0, 256, (40, 50), generator=g, dtype=torch.uint8)
+    out = torch.zeros(rows, 50, dtype=torch.uint8, device=ctx.device).view(torch.float8_e4m3fn)
+    plan.dispatch(x.to(ctx.device).view(torch.float8_e4m3fn), route, rows_out=out)
+    parts = [t.cpu() for t in (route.row_of_slot, route.counts, route.offsets)]
+    assert torch.equal(out.view(torch.uint8).cpu(), ref.dispatch(x, *parts, torch.zeros(rows, 50, dtype=torch.uint8)))
+
+
 def test_results_are_the_same_every_time(ctx, mrs):
     tokens = 20000
     g = torch.Generator(device=ctx.device).manual_seed(8)
@@ -579,6 +613,18 @@ def test_refusals(ctx, mrs):
     s = torch.zeros(8, 4, device=dev)
     with pytest.raises(mrs.MrsError, match="overlap"):
         plan.select_backward(s, torch.zeros(8, 2, dtype=torch.int32, device=dev), w, scores_grad_out=s)
+    ids = torch.zeros(8, 2, dtype=torch.int32, device=dev)
+    for bad in (mrs.RouteMap(ids, route.slot_of_row, route.counts, route.offsets),
+                mrs.RouteMap(route.row_of_slot, route.slot_of_row, route.slot_of_row, route.offsets),
+                mrs.RouteMap(route.row_of_slot, route.slot_of_row, route.offsets, route.offsets)):
+        with pytest.raises(mrs.MrsError, match="overlap"):
+            plan.order(ids, bad)
+    with pytest.raises(mrs.MrsError, match="overlap"):
+        plan.combine_backward(x, r, route, w, dweights_out=w)
+    with pytest.raises(mrs.MrsError, match="overlap"):
+        plan.select(s, ids_out=w.view(torch.int32), weights_out=w)
+    with pytest.raises(mrs.MrsError, match="overlap"):
+        plan.dispatch_backward(r[:, :2], route, x_grad_out=route.row_of_slot.view(torch.float32))
     with pytest.raises(ValueError, match="is on"):
         plan.dispatch(torch.zeros(8, 16), route)
     # no tokens: nothing to do, nothing refused

@@ -10,6 +10,13 @@ import wgpu_morton_code_radix_sort_test_amd as mrs
 from wgpu_morton_code_radix_sort_test_amd import _lib
 
 
+@pytest.fixture(autouse=True)
+def no_message_left_behind():
+    """Refusals leave a message with the thread until the next call that succeeds."""
+    yield
+    assert _lib.load_library().mrs_route_destroy(None) == _lib.MRS_OK
+
+
 def _desc(**kw):
     d = dict(tokens=100, experts=8, topk=2, align=1, gate=0, capacity=0, normalize=1, scale=1.0)
     d.update(kw)

@@ -428,7 +428,8 @@ class RoutePlan:
     picks their experts, `order` sorts the slots by expert, `dispatch` moves the tokens' rows into that
     order, `combine` brings them back weighted; the `*_backward` calls are the gradients.  An expert's rows start
     at a multiple of `align`; beyond `capacity` rows (0 = no limit) its later slots are dropped.  `gate`,
-    `normalize` and `scale` say how scores become weights (include/mrs.h).  One handle runs one `order` at a time."""
+    `normalize` and `scale` say how scores become weights (include/mrs.h).  One handle runs one `order` at a time.
+    Nothing is recorded for autograd: a training step makes the backward calls itself."""
 
     def __init__(self, ctx, tokens, experts, topk, align=1, capacity=0, gate=GATE_SOFTMAX, normalize=True, scale=1.0):
         self._h = None
@@ -504,6 +505,14 @@ class RoutePlan:
         rows = to_slot.numel()
         return _lib.RouteMapStruct(to_row.data_ptr(), to_slot.data_ptr(), counts.data_ptr(), offsets.data_ptr(), rows), rows
 
+    def _new(self, stream, shape, dtype):
+        """A tensor whose memory belongs to the stream the call writes it on: memory of another stream's may still be
+        written there by work of its previous owner."""
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
     def _on_stream(self, stream):
         return _raw_stream(self.device.index) if stream is None else stream.cuda_stream
 
@@ -532,20 +541,20 @@ class RoutePlan:
         return tokens, kind, ptr, ld
 
     # ---- calls -----------------------------------------------------------------------
-    def new_map(self, tokens=None):
-        """An unwritten RouteMap for `order` calls of `tokens` tokens (the plan's, by default)."""
+    def new_map(self, tokens=None, stream=None):
+        """An unwritten RouteMap for `order` calls of up to `tokens` tokens (the plan's, by default)."""
         tokens = self.tokens if tokens is None else tokens
-        make = lambda *shape: torch.empty(shape, dtype=torch.int32, device=self.device)  # noqa: E731
-        return RouteMap(make(tokens, self.topk), make(self.max_rows), make(self.experts), make(self.experts + 1))
+        shapes = ((tokens, self.topk), (self.max_rows,), (self.experts,), (self.experts + 1,))
+        return RouteMap(*(self._new(stream, shape, torch.int32) for shape in shapes))
 
     def select(self, scores, bias=None, ids_out=None, weights_out=None, stream=None):
         """`mrs_route_select`: the topk experts of every token and their weights, (ids int32, weights float32), both
         [tokens, topk], from scores [tokens, experts] (float32, float16 or bfloat16)."""
         tokens, kind, ptr, ld = self._scores(scores)
         if ids_out is None:
-            ids_out = torch.empty((tokens, self.topk), dtype=torch.int32, device=self.device)
+            ids_out = self._new(stream, (tokens, self.topk), torch.int32)
         if weights_out is None:
-            weights_out = torch.empty((tokens, self.topk), dtype=torch.float32, device=self.device)
+            weights_out = self._new(stream, (tokens, self.topk), torch.float32)
         _lib.check(
             self.lib.mrs_route_select(self._h, tokens, ptr, ld, kind, self._bias(bias),
                                       self._per_slot(ids_out, "ids_out", tokens, torch.int32),
@@ -557,7 +566,7 @@ class RoutePlan:
         """`mrs_route_select_backward`: the gradient of `scores`, of their type, from that of the weights."""
         tokens, kind, ptr, ld = self._scores(scores)
         if scores_grad_out is None:
-            scores_grad_out = scores.new_empty((tokens, self.experts))
+            scores_grad_out = self._new(stream, (tokens, self.experts), scores.dtype)
         grad_ptr, grad_ld = self._rows(scores_grad_out, "scores_grad_out", tokens, self.experts, scores.dtype)
         _lib.check(
             self.lib.mrs_route_select_backward(self._h, tokens, ptr, ld, kind, self._bias(bias),
@@ -573,7 +582,7 @@ class RoutePlan:
         tokens = self._slots(ids, "ids")
         ids_ptr = self._per_slot(ids, "ids", tokens, torch.int32)
         if map_out is None:
-            map_out = self.new_map(tokens)
+            map_out = self.new_map(tokens, stream)
         raw, _ = self._map(map_out, tokens)
         _lib.check(self.lib.mrs_route_order(self._h, tokens, ids_ptr, raw, self._on_stream(stream)))
         return map_out
@@ -586,7 +595,7 @@ class RoutePlan:
         raw, rows = self._map(route, tokens)
         x_ptr, ld_x = self._rows(x, "x", tokens, hidden, x.dtype)
         if rows_out is None:
-            rows_out = x.new_empty((rows, hidden))
+            rows_out = self._new(stream, (rows, hidden), x.dtype)
         out_ptr, ld_out = self._rows(rows_out, "rows_out", rows, hidden, x.dtype)
         _lib.check(self.lib.mrs_route_dispatch(self._h, tokens, raw, kind, hidden, x_ptr, ld_x, out_ptr, ld_out, self._on_stream(stream)))
         return rows_out
@@ -599,7 +608,7 @@ class RoutePlan:
         raw, rows = self._map(route, tokens)
         in_ptr, ld_in = self._rows(rows_grad, "rows_grad", rows, hidden, rows_grad.dtype)
         if x_grad_out is None:
-            x_grad_out = rows_grad.new_empty((tokens, hidden))
+            x_grad_out = self._new(stream, (tokens, hidden), rows_grad.dtype)
         out_ptr, ld_out = self._rows(x_grad_out, "x_grad_out", tokens, hidden, rows_grad.dtype)
         _lib.check(
             self.lib.mrs_route_dispatch_backward(self._h, tokens, raw, kind, hidden, in_ptr, ld_in, out_ptr, ld_out,
@@ -614,7 +623,7 @@ class RoutePlan:
         raw, count = self._map(route, tokens)
         in_ptr, ld_in = self._rows(rows, "rows", count, hidden, rows.dtype)
         if out is None:
-            out = rows.new_empty((tokens, hidden))
+            out = self._new(stream, (tokens, hidden), rows.dtype)
         out_ptr, ld_out = self._rows(out, "out", tokens, hidden, rows.dtype)
         _lib.check(
             self.lib.mrs_route_combine(self._h, tokens, raw, kind, hidden, in_ptr, ld_in,
@@ -632,9 +641,9 @@ class RoutePlan:
         grad_ptr, ld_grad = self._rows(out_grad, "out_grad", tokens, hidden, rows.dtype)
         in_ptr, ld_in = self._rows(rows, "rows", count, hidden, rows.dtype)
         if drows_out is None:
-            drows_out = rows.new_empty((count, hidden))
+            drows_out = self._new(stream, (count, hidden), rows.dtype)
         if dweights_out is None:
-            dweights_out = weights.new_empty((tokens, self.topk))
+            dweights_out = self._new(stream, (tokens, self.topk), torch.float32)
         out_ptr, ld_out = self._rows(drows_out, "drows_out", count, hidden, rows.dtype)
         _lib.check(
             self.lib.mrs_route_combine_backward(self._h, tokens, raw, kind, hidden, grad_ptr, ld_grad, in_ptr, ld_in,

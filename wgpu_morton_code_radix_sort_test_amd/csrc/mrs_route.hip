@@ -73,7 +73,7 @@ int check_matrix(const Matrix& m, const char* who, const char* name)
 // Whether two matrices share an element.  Column blocks of one buffer (same stride, disjoint columns) do not.
 bool overlap(const Matrix& a, const Matrix& b)
 {
-    if (a.rows == 0 || b.rows == 0) return false;
+    if (!a.p || !b.p || a.rows == 0 || b.rows == 0 || a.columns == 0 || b.columns == 0) return false;
     const uint64_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
     const uint64_t ea = pa + ((a.rows - 1) * a.stride + a.columns) * a.bytes;
     const uint64_t eb = pb + ((b.rows - 1) * b.stride + b.columns) * b.bytes;
@@ -84,9 +84,23 @@ bool overlap(const Matrix& a, const Matrix& b)
     return shift < a.columns * a.bytes || shift + b.columns * b.bytes > pitch;
 }
 
-int check_apart(const Matrix& a, const Matrix& b, const char* who, const char* names)
+// An array without rows of its own.
+Matrix flat(const void* p, uint64_t count) { return {p, 1, count, count, 4}; }
+
+// No output may share memory with an input or another output.
+struct Named {
+    Matrix m;
+    const char* name;
+};
+template <size_t OUT, size_t IN>
+int check_outputs(const Named (&out)[OUT], const Named (&in)[IN], const char* who)
 {
-    if (overlap(a, b)) return fail(MRS_ERR_INVALID_ARGUMENT, "%s: %s overlap", who, names);
+    for (size_t i = 0; i < OUT; ++i) {
+        for (size_t j = 0; j < IN; ++j)
+            if (overlap(out[i].m, in[j].m)) return fail(MRS_ERR_INVALID_ARGUMENT, "%s: %s and %s overlap", who, out[i].name, in[j].name);
+        for (size_t j = i + 1; j < OUT; ++j)
+            if (overlap(out[i].m, out[j].m)) return fail(MRS_ERR_INVALID_ARGUMENT, "%s: %s and %s overlap", who, out[i].name, out[j].name);
+    }
     return MRS_OK;
 }
 
@@ -220,6 +234,10 @@ extern "C" int mrs_route_select(mrs_route* route, uint64_t tokens, const void* s
     if (tokens == 0) return MRS_OK;
     if (int rc = check_ints(ids_dev, who, "ids")) return rc;
     if (int rc = check_ints(weights_dev, who, "weights")) return rc;
+    const uint64_t experts = static_cast<uint64_t>(route->desc.experts), slots = tokens * static_cast<uint64_t>(route->desc.topk);
+    const Named out[] = {{flat(ids_dev, slots), "ids"}, {flat(weights_dev, slots), "weights"}};
+    const Named in[] = {{{scores_dev, tokens, experts, ld_scores, element_bytes(type)}, "scores"}, {flat(bias_dev, experts), "bias"}};
+    if (int rc = check_outputs(out, in, who)) return rc;
     SelectArgs a = select_args(route, tokens, scores_dev, ld_scores, bias_dev);
     a.ids_out = ids_dev;
     a.weights_out = weights_dev;
@@ -238,13 +256,15 @@ extern "C" int mrs_route_select_backward(mrs_route* route, uint64_t tokens, cons
     if (tokens == 0) return MRS_OK;
     if (int rc = check_ints(ids_dev, who, "ids")) return rc;
     if (int rc = check_ints(weights_grad_dev, who, "weights_grad")) return rc;
-    const uint64_t experts = static_cast<uint64_t>(route->desc.experts), k = static_cast<uint64_t>(route->desc.topk);
+    const uint64_t experts = static_cast<uint64_t>(route->desc.experts), slots = tokens * static_cast<uint64_t>(route->desc.topk);
     const int bytes = element_bytes(type);
-    const Matrix scores{scores_dev, tokens, experts, ld_scores, bytes}, grad{scores_grad_dev, tokens, experts, ld_scores_grad, bytes};
-    if (int rc = check_matrix(grad, who, "scores_grad")) return rc;
-    if (int rc = check_apart(grad, scores, who, "scores_grad and scores")) return rc;
-    if (int rc = check_apart(grad, {ids_dev, tokens, k, k, 4}, who, "scores_grad and ids")) return rc;
-    if (int rc = check_apart(grad, {weights_grad_dev, tokens, k, k, 4}, who, "scores_grad and weights_grad")) return rc;
+    const Named out[] = {{{scores_grad_dev, tokens, experts, ld_scores_grad, bytes}, "scores_grad"}};
+    const Named in[] = {{{scores_dev, tokens, experts, ld_scores, bytes}, "scores"},
+                        {flat(bias_dev, experts), "bias"},
+                        {flat(ids_dev, slots), "ids"},
+                        {flat(weights_grad_dev, slots), "weights_grad"}};
+    if (int rc = check_matrix(out[0].m, who, "scores_grad")) return rc;
+    if (int rc = check_outputs(out, in, who)) return rc;
     SelectArgs a = select_args(route, tokens, scores_dev, ld_scores, bias_dev);
     a.ids = ids_dev;
     a.weights_grad = weights_grad_dev;
@@ -272,9 +292,16 @@ extern "C" int mrs_route_order(mrs_route* route, uint64_t tokens, const int32_t*
         if (int rc = check_ints(ids_dev, who, "ids")) return rc;
         if (int rc = check_ints(map->row_of_slot, who, "row_of_slot")) return rc;
     }
+    const uint64_t experts = static_cast<uint64_t>(route->desc.experts), slots = tokens * static_cast<uint64_t>(route->desc.topk);
+    const Named out[] = {{flat(map->row_of_slot, slots), "row_of_slot"},
+                         {flat(map->slot_of_row, map->rows), "slot_of_row"},
+                         {flat(map->counts, experts), "counts"},
+                         {flat(map->offsets, experts + 1), "offsets"}};
+    const Named in[] = {{flat(ids_dev, slots), "ids"}};
+    if (int rc = check_outputs(out, in, who)) return rc;
     OrderArgs a{};
     a.ids = ids_dev;
-    a.slots = tokens * static_cast<uint64_t>(route->desc.topk);
+    a.slots = slots;
     a.experts = static_cast<uint32_t>(route->desc.experts);
     a.align = static_cast<uint32_t>(route->desc.align);
     a.capacity = route->desc.capacity == 0 || route->desc.capacity > 0xFFFFFFFFull ? 0xFFFFFFFFu
@@ -300,10 +327,15 @@ extern "C" int mrs_route_dispatch(mrs_route* route, uint64_t tokens, const mrs_r
     if (int rc = check_map(route, tokens, map, true, who)) return rc;
     if (tokens == 0) return MRS_OK;
     const int bytes = element_bytes(type);
-    const Matrix x{x_dev, tokens, hidden, ld_x, bytes}, rows{rows_dev, map->rows, hidden, ld_rows, bytes};
-    if (int rc = check_matrix(x, who, "x")) return rc;
-    if (int rc = check_matrix(rows, who, "rows")) return rc;
-    if (int rc = check_apart(x, rows, who, "x and rows")) return rc;
+    const uint64_t experts = static_cast<uint64_t>(route->desc.experts), slots = tokens * static_cast<uint64_t>(route->desc.topk);
+    const Named out[] = {{{rows_dev, map->rows, hidden, ld_rows, bytes}, "rows"}};
+    const Named in[] = {{{x_dev, tokens, hidden, ld_x, bytes}, "x"},
+                        {flat(map->row_of_slot, slots), "row_of_slot"},
+                        {flat(map->counts, experts), "counts"},
+                        {flat(map->offsets, experts + 1), "offsets"}};
+    if (int rc = check_matrix(in[0].m, who, "x")) return rc;
+    if (int rc = check_matrix(out[0].m, who, "rows")) return rc;
+    if (int rc = check_outputs(out, in, who)) return rc;
     MoveArgs a = move_args(route, tokens, map, hidden);
     a.token_in = x_dev;
     a.ld_token_in = ld_x;
@@ -319,10 +351,14 @@ static int gather_sum(mrs_route* route, uint64_t tokens, const mrs_route_map* ma
                       uint64_t ld_out, const char* out_name, const char* who, void* stream)
 {
     const int bytes = element_bytes(type);
-    const Matrix rows{rows_dev, map->rows, hidden, ld_rows, bytes}, out{out_dev, tokens, hidden, ld_out, bytes};
-    if (int rc = check_matrix(rows, who, rows_name)) return rc;
-    if (int rc = check_matrix(out, who, out_name)) return rc;
-    if (int rc = check_apart(out, rows, who, "input and output rows")) return rc;
+    const uint64_t slots = tokens * static_cast<uint64_t>(route->desc.topk);
+    const Named out[] = {{{out_dev, tokens, hidden, ld_out, bytes}, out_name}};
+    const Named in[] = {{{rows_dev, map->rows, hidden, ld_rows, bytes}, rows_name},
+                        {flat(map->row_of_slot, slots), "row_of_slot"},
+                        {flat(weights_dev, slots), "weights"}};
+    if (int rc = check_matrix(in[0].m, who, rows_name)) return rc;
+    if (int rc = check_matrix(out[0].m, who, out_name)) return rc;
+    if (int rc = check_outputs(out, in, who)) return rc;
     MoveArgs a = move_args(route, tokens, map, hidden);
     a.rows_in = rows_dev;
     a.ld_rows_in = ld_rows;
@@ -379,15 +415,19 @@ extern "C" int mrs_route_combine_backward(mrs_route* route, uint64_t tokens, con
     if (int rc = check_ints(weights_dev, who, "weights")) return rc;
     if (int rc = check_ints(weights_grad_dev, who, "weights_grad")) return rc;
     const int bytes = element_bytes(type);
-    const uint64_t k = static_cast<uint64_t>(route->desc.topk);
-    const Matrix grad{out_grad_dev, tokens, hidden, ld_out_grad, bytes}, rows{rows_dev, map->rows, hidden, ld_rows, bytes},
-        rows_grad{rows_grad_dev, map->rows, hidden, ld_rows_grad, bytes}, weights{weights_dev, tokens, k, k, 4};
-    if (int rc = check_matrix(grad, who, "out_grad")) return rc;
-    if (int rc = check_matrix(rows, who, "rows")) return rc;
-    if (int rc = check_matrix(rows_grad, who, "rows_grad")) return rc;
-    if (int rc = check_apart(rows_grad, rows, who, "rows_grad and rows")) return rc;
-    if (int rc = check_apart(rows_grad, grad, who, "rows_grad and out_grad")) return rc;
-    if (int rc = check_apart(rows_grad, weights, who, "rows_grad and weights")) return rc;
+    const uint64_t experts = static_cast<uint64_t>(route->desc.experts), slots = tokens * static_cast<uint64_t>(route->desc.topk);
+    const Named out[] = {{{rows_grad_dev, map->rows, hidden, ld_rows_grad, bytes}, "rows_grad"},
+                         {flat(weights_grad_dev, slots), "weights_grad"}};
+    const Named in[] = {{{out_grad_dev, tokens, hidden, ld_out_grad, bytes}, "out_grad"},
+                        {{rows_dev, map->rows, hidden, ld_rows, bytes}, "rows"},
+                        {flat(weights_dev, slots), "weights"},
+                        {flat(map->row_of_slot, slots), "row_of_slot"},
+                        {flat(map->counts, experts), "counts"},
+                        {flat(map->offsets, experts + 1), "offsets"}};
+    if (int rc = check_matrix(in[0].m, who, "out_grad")) return rc;
+    if (int rc = check_matrix(in[1].m, who, "rows")) return rc;
+    if (int rc = check_matrix(out[0].m, who, "rows_grad")) return rc;
+    if (int rc = check_outputs(out, in, who)) return rc;
     MoveArgs a = move_args(route, tokens, map, hidden);
     a.token_in = out_grad_dev;
     a.ld_token_in = ld_out_grad;
