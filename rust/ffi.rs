@@ -27,6 +27,40 @@ pub struct mrs_comm { _private: [u8; 0] }
 pub struct mrs_dist { _private: [u8; 0] }
 #[repr(C)]
 pub struct mrs_splitter { _private: [u8; 0] }
+#[repr(C)]
+pub struct mrs_route { _private: [u8; 0] }
+
+pub const GATE_SOFTMAX: i32 = 0;
+pub const GATE_SIGMOID: i32 = 1;
+pub const TYPE_F32: i32 = 0;
+pub const TYPE_F16: i32 = 1;
+pub const TYPE_BF16: i32 = 2;
+pub const TYPE_8BIT: i32 = 3;
+
+/// `mrs_route_desc`: tokens routed to experts.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mrs_route_desc {
+    pub tokens: u64,
+    pub experts: i32,
+    pub topk: i32,
+    pub align: i32,
+    pub gate: i32,
+    pub capacity: u64,
+    pub normalize: i32,
+    pub scale: f32,
+}
+
+/// `mrs_route_map`: device arrays of the caller.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct mrs_route_map {
+    pub row_of_slot: *mut i32,
+    pub slot_of_row: *mut i32,
+    pub counts: *mut i32,
+    pub offsets: *mut i32,
+    pub rows: u64,
+}
 
 /// `mrs_dist_desc`: the sharded sort of one rank.
 #[repr(C)]
@@ -184,6 +218,29 @@ extern "C" {
                              prefixes: *mut u64) -> c_int;
     pub fn mrs_splitter_feed(sp: *mut mrs_splitter, counts: *const u64) -> c_int;
     pub fn mrs_splitter_get(sp: *const mrs_splitter, out: *mut mrs_split_result) -> c_int;
+    pub fn mrs_route_create(ctx: *mut mrs_context, desc: *const mrs_route_desc, out: *mut *mut mrs_route) -> c_int;
+    pub fn mrs_route_destroy(route: *mut mrs_route) -> c_int;
+    pub fn mrs_route_max_rows(desc: *const mrs_route_desc, rows: *mut u64) -> c_int;
+    pub fn mrs_route_select(route: *mut mrs_route, tokens: u64, scores_dev: *const c_void, ld_scores: u64, type_: i32,
+                            bias_dev: *const f32, ids_dev: *mut i32, weights_dev: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn mrs_route_select_backward(route: *mut mrs_route, tokens: u64, scores_dev: *const c_void, ld_scores: u64, type_: i32,
+                                     bias_dev: *const f32, ids_dev: *const i32, weights_grad_dev: *const f32,
+                                     scores_grad_dev: *mut c_void, ld_scores_grad: u64, stream: *mut c_void) -> c_int;
+    pub fn mrs_route_order(route: *mut mrs_route, tokens: u64, ids_dev: *const i32, map: *const mrs_route_map,
+                           stream: *mut c_void) -> c_int;
+    pub fn mrs_route_dispatch(route: *mut mrs_route, tokens: u64, map: *const mrs_route_map, type_: i32, hidden: u64,
+                              x_dev: *const c_void, ld_x: u64, rows_dev: *mut c_void, ld_rows: u64,
+                              stream: *mut c_void) -> c_int;
+    pub fn mrs_route_dispatch_backward(route: *mut mrs_route, tokens: u64, map: *const mrs_route_map, type_: i32, hidden: u64,
+                                       rows_grad_dev: *const c_void, ld_rows_grad: u64, x_grad_dev: *mut c_void,
+                                       ld_x_grad: u64, stream: *mut c_void) -> c_int;
+    pub fn mrs_route_combine(route: *mut mrs_route, tokens: u64, map: *const mrs_route_map, type_: i32, hidden: u64,
+                             rows_dev: *const c_void, ld_rows: u64, weights_dev: *const f32, out_dev: *mut c_void,
+                             ld_out: u64, stream: *mut c_void) -> c_int;
+    pub fn mrs_route_combine_backward(route: *mut mrs_route, tokens: u64, map: *const mrs_route_map, type_: i32, hidden: u64,
+                                      out_grad_dev: *const c_void, ld_out_grad: u64, rows_dev: *const c_void, ld_rows: u64,
+                                      weights_dev: *const f32, rows_grad_dev: *mut c_void, ld_rows_grad: u64,
+                                      weights_grad_dev: *mut f32, stream: *mut c_void) -> c_int;
     pub fn mrs_generate_points(ctx: *mut mrs_context, seed: u64, n: u64, xyz_dev: *mut f32,
                                stream: *mut c_void) -> c_int;
     pub fn mrs_generate_u32(ctx: *mut mrs_context, seed: u64, stream_id: u64, n: u64, out_dev: *mut u32,
