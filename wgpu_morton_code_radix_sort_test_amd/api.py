@@ -513,6 +513,20 @@ class RoutePlan:
         with torch.cuda.stream(stream):
             return torch.empty(shape, dtype=dtype, device=self.device)
 
+    def _slots_out(self, t, name, tokens, dtype, stream):
+        """A caller's output for every slot, checked, or a new one; and its pointer."""
+        if t is not None:
+            return t, self._per_slot(t, name, tokens, dtype)
+        t = self._new(stream, (tokens, self.topk), dtype)
+        return t, t.data_ptr()
+
+    def _rows_out(self, t, name, rows, hidden, dtype, stream):
+        """A caller's output matrix, checked, or a new one; its pointer and row stride."""
+        if t is not None:
+            return (t, *self._rows(t, name, rows, hidden, dtype))
+        t = self._new(stream, (rows, hidden), dtype)
+        return t, t.data_ptr(), hidden
+
     def _on_stream(self, stream):
         return _raw_stream(self.device.index) if stream is None else stream.cuda_stream
 
@@ -551,30 +565,25 @@ class RoutePlan:
         """`mrs_route_select`: the topk experts of every token and their weights, (ids int32, weights float32), both
         [tokens, topk], from scores [tokens, experts] (float32, float16 or bfloat16)."""
         tokens, kind, ptr, ld = self._scores(scores)
-        if ids_out is None:
-            ids_out = self._new(stream, (tokens, self.topk), torch.int32)
-        if weights_out is None:
-            weights_out = self._new(stream, (tokens, self.topk), torch.float32)
+        ids_out, ids_ptr = self._slots_out(ids_out, "ids_out", tokens, torch.int32, stream)
+        weights_out, weights_ptr = self._slots_out(weights_out, "weights_out", tokens, torch.float32, stream)
         _lib.check(
-            self.lib.mrs_route_select(self._h, tokens, ptr, ld, kind, self._bias(bias),
-                                      self._per_slot(ids_out, "ids_out", tokens, torch.int32),
-                                      self._per_slot(weights_out, "weights_out", tokens, torch.float32), self._on_stream(stream))
+            self.lib.mrs_route_select(self._h, tokens, ptr, ld, kind, self._bias(bias), ids_ptr, weights_ptr,
+                                      self._on_stream(stream))
         )
         return ids_out, weights_out
 
     def select_backward(self, scores, ids, weights_grad, bias=None, scores_grad_out=None, stream=None):
         """`mrs_route_select_backward`: the gradient of `scores`, of their type, from that of the weights."""
         tokens, kind, ptr, ld = self._scores(scores)
-        if scores_grad_out is None:
-            scores_grad_out = self._new(stream, (tokens, self.experts), scores.dtype)
-        grad_ptr, grad_ld = self._rows(scores_grad_out, "scores_grad_out", tokens, self.experts, scores.dtype)
+        out, grad_ptr, grad_ld = self._rows_out(scores_grad_out, "scores_grad_out", tokens, self.experts, scores.dtype, stream)
         _lib.check(
             self.lib.mrs_route_select_backward(self._h, tokens, ptr, ld, kind, self._bias(bias),
                                                self._per_slot(ids, "ids", tokens, torch.int32),
                                                self._per_slot(weights_grad, "weights_grad", tokens, torch.float32),
                                                grad_ptr, grad_ld, self._on_stream(stream))
         )
-        return scores_grad_out
+        return out
 
     def order(self, ids, map_out=None, stream=None):
         """`mrs_route_order`: a RouteMap of the slots sorted by ids [tokens, topk] (int32; ids outside [0, experts)
@@ -591,25 +600,24 @@ class RoutePlan:
         """`mrs_route_dispatch`: x [tokens, hidden] in expert order, [rows, hidden].  Rows behind the last segment are
         left as they are: in an own `rows_out` that is what was there, in a new tensor anything."""
         kind = self._row_type(x, "x", eight_bits=True)
-        tokens, hidden = x.size(0), x.size(1)
+        tokens, hidden = x.shape
         raw, rows = self._map(route, tokens)
         x_ptr, ld_x = self._rows(x, "x", tokens, hidden, x.dtype)
-        if rows_out is None:
-            rows_out = self._new(stream, (rows, hidden), x.dtype)
-        out_ptr, ld_out = self._rows(rows_out, "rows_out", rows, hidden, x.dtype)
-        _lib.check(self.lib.mrs_route_dispatch(self._h, tokens, raw, kind, hidden, x_ptr, ld_x, out_ptr, ld_out, self._on_stream(stream)))
+        rows_out, out_ptr, ld_out = self._rows_out(rows_out, "rows_out", rows, hidden, x.dtype, stream)
+        _lib.check(self.lib.mrs_route_dispatch(self._h, tokens, raw, kind, hidden, x_ptr, ld_x, out_ptr, ld_out,
+                                               self._on_stream(stream)))
         return rows_out
 
     def dispatch_backward(self, rows_grad, route, x_grad_out=None, tokens=None, stream=None):
-        """`mrs_route_dispatch_backward`: the gradient of x [tokens, hidden]; `tokens` by default those of the map."""
+        """`mrs_route_dispatch_backward`: the gradient of x [tokens, hidden].  `tokens`: those that were ordered, where the map
+        has room for more (its own by default)."""
         kind = self._row_type(rows_grad, "rows_grad")
         hidden = rows_grad.size(1)
-        tokens = self._tokens_of(route, tokens)
+        if tokens is None:
+            tokens = route.row_of_slot.numel() // self.topk
         raw, rows = self._map(route, tokens)
         in_ptr, ld_in = self._rows(rows_grad, "rows_grad", rows, hidden, rows_grad.dtype)
-        if x_grad_out is None:
-            x_grad_out = self._new(stream, (tokens, hidden), rows_grad.dtype)
-        out_ptr, ld_out = self._rows(x_grad_out, "x_grad_out", tokens, hidden, rows_grad.dtype)
+        x_grad_out, out_ptr, ld_out = self._rows_out(x_grad_out, "x_grad_out", tokens, hidden, rows_grad.dtype, stream)
         _lib.check(
             self.lib.mrs_route_dispatch_backward(self._h, tokens, raw, kind, hidden, in_ptr, ld_in, out_ptr, ld_out,
                                                  self._on_stream(stream))
@@ -622,9 +630,7 @@ class RoutePlan:
         tokens, hidden = self._slots(weights, "weights"), rows.size(1)
         raw, count = self._map(route, tokens)
         in_ptr, ld_in = self._rows(rows, "rows", count, hidden, rows.dtype)
-        if out is None:
-            out = self._new(stream, (tokens, hidden), rows.dtype)
-        out_ptr, ld_out = self._rows(out, "out", tokens, hidden, rows.dtype)
+        out, out_ptr, ld_out = self._rows_out(out, "out", tokens, hidden, rows.dtype, stream)
         _lib.check(
             self.lib.mrs_route_combine(self._h, tokens, raw, kind, hidden, in_ptr, ld_in,
                                        self._per_slot(weights, "weights", tokens, torch.float32), out_ptr, ld_out,
@@ -640,18 +646,11 @@ class RoutePlan:
         raw, count = self._map(route, tokens)
         grad_ptr, ld_grad = self._rows(out_grad, "out_grad", tokens, hidden, rows.dtype)
         in_ptr, ld_in = self._rows(rows, "rows", count, hidden, rows.dtype)
-        if drows_out is None:
-            drows_out = self._new(stream, (count, hidden), rows.dtype)
-        if dweights_out is None:
-            dweights_out = self._new(stream, (tokens, self.topk), torch.float32)
-        out_ptr, ld_out = self._rows(drows_out, "drows_out", count, hidden, rows.dtype)
+        weights_ptr = self._per_slot(weights, "weights", tokens, torch.float32)
+        drows_out, out_ptr, ld_out = self._rows_out(drows_out, "drows_out", count, hidden, rows.dtype, stream)
+        dweights_out, sums_ptr = self._slots_out(dweights_out, "dweights_out", tokens, torch.float32, stream)
         _lib.check(
             self.lib.mrs_route_combine_backward(self._h, tokens, raw, kind, hidden, grad_ptr, ld_grad, in_ptr, ld_in,
-                                                self._per_slot(weights, "weights", tokens, torch.float32), out_ptr, ld_out,
-                                                self._per_slot(dweights_out, "dweights_out", tokens, torch.float32),
-                                                self._on_stream(stream))
+                                                weights_ptr, out_ptr, ld_out, sums_ptr, self._on_stream(stream))
         )
         return drows_out, dweights_out
-
-    def _tokens_of(self, route, tokens):
-        return route.row_of_slot.numel() // self.topk if tokens is None else tokens

@@ -242,7 +242,7 @@ extern "C" int mrs_route_select(mrs_route* route, uint64_t tokens, const void* s
     a.ids_out = ids_dev;
     a.weights_out = weights_dev;
     const ProfilerRange range("Select");
-    return launch_route_select(type, a, route->ctx->num_cus, static_cast<hipStream_t>(stream));
+    return launch_route_select(type, a, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int mrs_route_select_backward(mrs_route* route, uint64_t tokens, const void* scores_dev, uint64_t ld_scores,
@@ -271,7 +271,7 @@ extern "C" int mrs_route_select_backward(mrs_route* route, uint64_t tokens, cons
     a.scores_grad = scores_grad_dev;
     a.ld_scores_grad = ld_scores_grad;
     const ProfilerRange range("Select backward");
-    return launch_route_select_backward(type, a, route->ctx->num_cus, static_cast<hipStream_t>(stream));
+    return launch_route_select_backward(type, a, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int mrs_route_order(mrs_route* route, uint64_t tokens, const int32_t* ids_dev, const mrs_route_map* map, void* stream)
@@ -342,7 +342,7 @@ extern "C" int mrs_route_dispatch(mrs_route* route, uint64_t tokens, const mrs_r
     a.rows_out = rows_dev;
     a.ld_rows_out = ld_rows;
     const ProfilerRange range("Dispatch");
-    return launch_route_dispatch(bytes, a, route->ctx->num_cus, static_cast<hipStream_t>(stream));
+    return launch_route_dispatch(bytes, a, static_cast<hipStream_t>(stream));
 }
 
 // Token rows as sums of expert rows: combine, and dispatch's gradient (no weights).
@@ -365,7 +365,7 @@ static int gather_sum(mrs_route* route, uint64_t tokens, const mrs_route_map* ma
     a.weights = weights_dev;
     a.token_out = out_dev;
     a.ld_token_out = ld_out;
-    return launch_route_combine(type, a, route->ctx->num_cus, static_cast<hipStream_t>(stream));
+    return launch_route_combine(type, a, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int mrs_route_dispatch_backward(mrs_route* route, uint64_t tokens, const mrs_route_map* map, int32_t type,
@@ -438,5 +438,5 @@ extern "C" int mrs_route_combine_backward(mrs_route* route, uint64_t tokens, con
     a.ld_rows_out = ld_rows_grad;
     a.weights_grad = weights_grad_dev;
     const ProfilerRange range("Combine backward");
-    return launch_route_combine_backward(type, a, route->ctx->num_cus, static_cast<hipStream_t>(stream));
+    return launch_route_combine_backward(type, a, static_cast<hipStream_t>(stream));
 }

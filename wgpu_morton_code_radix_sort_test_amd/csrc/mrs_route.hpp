@@ -73,12 +73,12 @@ struct MoveArgs {
     float* weights_grad;
 };
 
-int launch_route_select(int type, const SelectArgs& a, int num_cus, hipStream_t s);
-int launch_route_select_backward(int type, const SelectArgs& a, int num_cus, hipStream_t s);
+int launch_route_select(int type, const SelectArgs& a, hipStream_t s);
+int launch_route_select_backward(int type, const SelectArgs& a, hipStream_t s);
 int launch_route_order(const OrderArgs& a, hipStream_t s);
-int launch_route_dispatch(int element_bytes, const MoveArgs& a, int num_cus, hipStream_t s);
-int launch_route_combine(int type, const MoveArgs& a, int num_cus, hipStream_t s);  // weights null: all 1
-int launch_route_combine_backward(int type, const MoveArgs& a, int num_cus, hipStream_t s);
+int launch_route_dispatch(int element_bytes, const MoveArgs& a, hipStream_t s);
+int launch_route_combine(int type, const MoveArgs& a, hipStream_t s);  // weights null: all 1
+int launch_route_combine_backward(int type, const MoveArgs& a, hipStream_t s);
 
 // ---- device side ------------------------------------------------------------------------------
 

@@ -7,8 +7,9 @@
 // the equal lanes below; a scan over the waves' counters gives the rank inside the tile.  No
 // atomics decide an order, so rows are the same every time.
 //
-// Up to kSmallSlots slots one workgroup does everything in one launch (512 slots, 256 experts: 4.0 us); what bounds it is
-// the launch and the chain of LDS accesses and barriers.  Above, a first launch counts tiles, and in a second one every
+// Up to kSmallSlots slots one workgroup does everything in one launch (256 experts: 4.0 us for 512 slots, 7.3 for 4096;
+// 8192 slots took 11.3, two launches 10.1); what bounds it is the launch and the chain of LDS accesses and
+// barriers.  Above, a first launch counts tiles, and in a second one every
 // workgroup adds up the counts of the tiles before its own by itself (at most 256 tiles of `experts` counts, read from
 // L2) instead of waiting for a scan launch between the two.  2^20 slots, 256 experts: 17 us, 4 of them for the counts, about 3 each for
 // adding them up and for the writes to slot_of_row in runs of some 16 rows.
@@ -22,7 +23,7 @@ constexpr uint32_t kWaves = 16;
 constexpr uint32_t kThreads = kWaves * 64;
 constexpr uint32_t kMaxExperts = MRS_ROUTE_MAX_EXPERTS;
 static_assert(kMaxExperts <= kThreads, "one thread per expert in the scans");
-constexpr uint32_t kSmallSlots = kThreads * 8;
+constexpr uint32_t kSmallSlots = kThreads * 4;
 constexpr uint32_t kTileR = 4;
 constexpr uint32_t kTileSlots = kThreads * kTileR;
 
@@ -320,8 +321,10 @@ int launch_route_order(const OrderArgs& a, hipStream_t s)
     if (a.slots <= kSmallSlots) {
         if (a.slots <= kThreads)
             hipLaunchKernelGGL(route_order_small_kernel<1>, dim3(1), dim3(kThreads), 0, s, a, bits);
+        else if (a.slots <= 2 * kThreads)
+            hipLaunchKernelGGL(route_order_small_kernel<2>, dim3(1), dim3(kThreads), 0, s, a, bits);
         else
-            hipLaunchKernelGGL(route_order_small_kernel<8>, dim3(1), dim3(kThreads), 0, s, a, bits);
+            hipLaunchKernelGGL(route_order_small_kernel<4>, dim3(1), dim3(kThreads), 0, s, a, bits);
         MRS_CHECK_LAUNCH("route_order_small_kernel");
         return MRS_OK;
     }

@@ -6,28 +6,27 @@
 
 #include "mrs_route.hpp"
 
-
 namespace mrs {
 
 namespace {
 
-constexpr uint32_t kMoveThreads = 128;   // dispatch
-constexpr uint32_t kSumThreads = 1024;   // combine and its gradient: a workgroup covers whole rows
+constexpr uint32_t kMoveThreads = 128;     // dispatch
+constexpr uint32_t kSumThreads = 1024;     // combine and its gradient: a workgroup covers whole rows
 constexpr uint32_t kMaxBlocks = 1u << 20;  // more work than that is looped over
 // Rows that cannot stay in the 256 MiB memory-side cache until somebody reads them again are streamed past the caches.
 constexpr uint64_t kStreamBytes = 256ull << 20;
 
-// How a launch cuts its work.  A group of `lanes` lanes -- a power of two up to a wave's 64, enough for the row if they can be --
+// How a launch cuts its work.  A group of lanes -- a power of two up to a wave's 64, enough for the row if they can be --
 // takes a piece of a row, a 16-byte vector a lane.
 struct Cut {
     uint32_t lanes_log2;
-    uint32_t vectors;     // whole 16-byte vectors of a row
-    uint32_t pieces;      // of a row
-    uint32_t items;       // what groups take: tokens * pieces, or tokens * token_waves
-    uint32_t token_waves; // combine's gradient: waves that share a token's pieces evenly, a power of two
-    uint32_t blocks;      // workgroups for the items
-    uint32_t pad_blocks;  // workgroups before them that zero the rows between segments' ends
-    uint32_t pad_split;   // of these, how many share an expert
+    uint32_t vectors;      // whole 16-byte vectors of a row
+    uint32_t pieces;       // of a row
+    uint32_t items;        // what groups take: tokens * pieces, or tokens * token_waves
+    uint32_t token_waves;  // combine's gradient: waves that share a token's pieces evenly, a power of two
+    uint32_t blocks;       // workgroups for the items
+    uint32_t pad_blocks;   // workgroups before them that zero the rows that fill segments up
+    uint32_t pad_split;    // of these, how many share an expert
 };
 
 int cut_rows(const MoveArgs& a, uint32_t element_bytes, uint32_t threads, bool whole_tokens, bool pads, Cut* out)
@@ -436,21 +435,21 @@ int start_combine_backward(const MoveArgs& a, hipStream_t s)
 
 }  // namespace
 
-int launch_route_dispatch(int element_bytes, const MoveArgs& a, int, hipStream_t s)
+int launch_route_dispatch(int element_bytes, const MoveArgs& a, hipStream_t s)
 {
     if (element_bytes == 1) return start_dispatch<uint8_t>(a, s);
     if (element_bytes == 2) return start_dispatch<uint16_t>(a, s);
     return start_dispatch<uint32_t>(a, s);
 }
 
-int launch_route_combine(int type, const MoveArgs& a, int, hipStream_t s)
+int launch_route_combine(int type, const MoveArgs& a, hipStream_t s)
 {
     if (type == MRS_TYPE_F32) return a.weights ? start_combine<float, true>(a, s) : start_combine<float, false>(a, s);
     if (type == MRS_TYPE_F16) return a.weights ? start_combine<_Float16, true>(a, s) : start_combine<_Float16, false>(a, s);
     return a.weights ? start_combine<__bf16, true>(a, s) : start_combine<__bf16, false>(a, s);
 }
 
-int launch_route_combine_backward(int type, const MoveArgs& a, int, hipStream_t s)
+int launch_route_combine_backward(int type, const MoveArgs& a, hipStream_t s)
 {
     if (type == MRS_TYPE_F32) return start_combine_backward<float>(a, s);
     if (type == MRS_TYPE_F16) return start_combine_backward<_Float16>(a, s);

@@ -247,7 +247,7 @@ __device__ __forceinline__ void take_largest(double (&list)[8], uint32_t topk, u
 // of the time.  16 lanes a row and 16 columns a lane take 35 us; reading the next row ahead gains nothing.
 template <typename T, uint32_t L, uint32_t V, bool FEW, bool WHOLE>
 __global__ __launch_bounds__(kThreads, 4) void route_select_kernel(const T* __restrict__ scores, const float* __restrict__ bias,
-                                                                const SelectArgs a)
+                                                                   const SelectArgs a)
 {
     using S = Share<T, L, V>;
     constexpr uint32_t kGroups = kThreads / L;
@@ -322,9 +322,10 @@ __global__ __launch_bounds__(kThreads, 4) void route_select_kernel(const T* __re
     }
 }
 
-// The gradient: 18.5 us for 65536 tokens, 8 of 256 scores.  It writes whole rows (64 MiB) and reads the chosen scores, which lie
-// in most of a row's cache lines; 8 to 32 lanes a row take the same.  The slots' derivatives are worked out by the first lanes of the group and laid into a row in LDS, which is written
-// out, less p[e] times their sum where the softmax runs over the whole row.
+// The gradient: 18.5 us for 65536 tokens, 8 of 256 scores.  It writes whole rows (64 MiB) and reads the chosen scores,
+// which lie in most of a row's cache lines; 8 to 32 lanes a row take the same.  The slots' derivatives are worked out
+// by the first lanes of the group and laid into a row in LDS, which is written out, less p[e] times their sum where the
+// softmax runs over the whole row.
 template <typename T, uint32_t L, uint32_t V, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void route_select_backward_kernel(const T* __restrict__ scores, const float* __restrict__ bias,
                                                                          T* __restrict__ scores_grad, const SelectArgs a)
@@ -474,7 +475,7 @@ void choose_backward(const SelectArgs& a, hipStream_t s)
 
 }  // namespace
 
-int launch_route_select(int type, const SelectArgs& a, int, hipStream_t s)
+int launch_route_select(int type, const SelectArgs& a, hipStream_t s)
 {
     if (type == MRS_TYPE_F32)
         choose<float>(a, s);
@@ -486,7 +487,7 @@ int launch_route_select(int type, const SelectArgs& a, int, hipStream_t s)
     return MRS_OK;
 }
 
-int launch_route_select_backward(int type, const SelectArgs& a, int, hipStream_t s)
+int launch_route_select_backward(int type, const SelectArgs& a, hipStream_t s)
 {
     if (type == MRS_TYPE_F32)
         choose_backward<float>(a, s);
