@@ -287,7 +287,7 @@ def untouched(wide, hidden, shift):
 
 SHAPES = [(1, 1, 1, 1, 1), (1, 4, 2, 8, 4), (2, 3, 3, 7, 1), (5, 8, 2, 64, 16), (7, 5, 5, 15, 3), (9, 4, 1, 16, 1), (33, 8, 4, 100, 8),
           (64, 16, 8, 129, 1), (3, 64, 32, 250, 2), (20, 6, 6, 513, 4), (6, 9, 9, 1024, 128), (11, 8, 8, 1109, 1), (4, 7, 16, 2050, 7),
-          (3, 256, 8, 4096, 16), (2, 3, 17, 8200, 1), (300, 8, 3, 33, 64)]
+          (3, 256, 8, 4096, 16), (2, 3, 17, 8200, 1), (300, 8, 3, 33, 64), (2, 4, 8, 6368, 16), (5, 300, 9, 227, 8)]
 
 
 @pytest.mark.parametrize("pad,shift", [(0, 0), (5, 1), (16, 8)])
@@ -345,7 +345,8 @@ def test_combine_and_dispatch_backward(ctx, mrs, tokens, experts, topk, hidden, 
 @pytest.mark.parametrize("tokens,experts,topk,hidden,align", SHAPES)
 def test_combine_backward(ctx, mrs, tokens, experts, topk, hidden, align, dtype, pad, shift):
     """rows: a product rounded to 32 bits, then to the type.  weights: a lane adds at most hidden / 64 + 8 products (rows of up to 64
-    vectors of 16 bytes: 8), the lanes' sums meet in at most 8 additions more."""
+    vectors of 16 bytes: 8), the lanes' sums meet in 6 additions more.  Where n of up to 16 waves share a row, that is one of
+    n * 64 vectors at least, a lane's part is that much shorter, which makes room for the n - 1 additions of their sums."""
     plan, route, rows, g = make_route(mrs, ctx, tokens, experts, topk, align, seed=3)
     x, dout = torch.randn(rows, hidden, generator=g).to(dtype), torch.randn(tokens, hidden, generator=g).to(dtype)
     w = torch.randn(tokens, topk, generator=g)

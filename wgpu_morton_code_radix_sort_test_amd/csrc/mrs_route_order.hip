@@ -8,11 +8,12 @@
 // atomics decide an order, so rows are the same every time.
 //
 // Up to kSmallSlots slots one workgroup does everything in one launch (256 experts: 4.0 us for 512 slots, 7.3 for 4096;
-// 8192 slots took 11.3, two launches 10.1); what bounds it is the launch and the chain of LDS accesses and
-// barriers.  Above, a first launch counts tiles, and in a second one every
-// workgroup adds up the counts of the tiles before its own by itself (at most 256 tiles of `experts` counts, read from
-// L2) instead of waiting for a scan launch between the two.  2^20 slots, 256 experts: 17 us, 4 of them for the counts, about 3 each for
-// adding them up and for the writes to slot_of_row in runs of some 16 rows.
+// 8192 took 11.3); what bounds it is the launch and the chain of LDS accesses and barriers.  Up to kDirectSlots one launch
+// of several workgroups, each of which counts all slots by itself (16384 slots 9.2 us, with two launches 10.5; 65536 14.2
+// and 11.0).  Above, a first launch counts tiles, and in a second one every workgroup adds up the counts of the tiles
+// before its own by itself (at most 256 tiles of `experts` counts, read from L2) instead of waiting for a scan launch
+// between the two.  2^20 slots, 256 experts: 17 us, 4 of them for the counts, about 3 each for adding them up and for the
+// writes to slot_of_row in runs of some 16 rows.
 #include "mrs_route.hpp"
 
 namespace mrs {
@@ -24,14 +25,15 @@ constexpr uint32_t kThreads = kWaves * 64;
 constexpr uint32_t kMaxExperts = MRS_ROUTE_MAX_EXPERTS;
 static_assert(kMaxExperts <= kThreads, "one thread per expert in the scans");
 constexpr uint32_t kSmallSlots = kThreads * 4;
+constexpr uint32_t kDirectSlots = 16384;
 constexpr uint32_t kTileR = 4;
 constexpr uint32_t kTileSlots = kThreads * kTileR;
 
 struct OrderShared {
     alignas(4) uint16_t wave_count[kWaves][kMaxExperts];  // slots per wave, then those of the waves before
-    uint32_t row[kMaxExperts];                 // first row of the expert in this tile
-    uint32_t room[kMaxExperts];                // rows it may still take
-    uint32_t fill[kMaxExperts];                // first row of its segment without a slot
+    uint32_t row[kMaxExperts];                            // first row of the expert in this tile
+    uint32_t room[kMaxExperts];                           // rows it may still take
+    uint32_t fill[kMaxExperts];                           // first row of its segment without a slot
     uint32_t fill_end[kMaxExperts];
     uint32_t wave_sum[kWaves];
 };
@@ -88,8 +90,8 @@ __device__ __forceinline__ void load_experts(const OrderArgs& a, uint64_t first,
         if (expert[i] > a.experts) expert[i] = a.experts;
 }
 
-// Ranks slots inside their wave's stretch, and leaves its counts in the wave's row of counters.  Only the wave itself touches that
-// row, and its LDS accesses stay in order: no barrier here.
+// Ranks slots inside their wave's stretch, and leaves its counts in the wave's row of counters.  Only the wave itself
+// touches that row, and its LDS accesses stay in order: no barrier here.
 template <uint32_t R>
 __device__ __forceinline__ void rank_in_waves(const OrderArgs& a, OrderShared& sh, uint32_t bits, const uint32_t (&expert)[R],
                                               uint32_t (&rank)[R])
@@ -151,7 +153,8 @@ __device__ __forceinline__ void write_rows(const OrderArgs& a, const OrderShared
 
 // Rows without a slot: what fills the segments up, shared out by expert among `blocks` workgroups and inside one among
 // groups of lanes as wide as a segment can need, and everything behind the last segment.
-__device__ __forceinline__ void mark_empty_rows(const OrderArgs& a, const OrderShared& sh, uint32_t end, uint32_t block, uint32_t blocks)
+__device__ __forceinline__ void mark_empty_rows(const OrderArgs& a, const OrderShared& sh, uint32_t end, uint32_t block,
+                                                uint32_t blocks)
 {
     if (a.align > 1) {
         uint32_t lanes = 64;
@@ -216,26 +219,12 @@ __global__ __launch_bounds__(kThreads) void route_order_count_kernel(const Order
     if (tid < a.experts) a.tile_counts[static_cast<uint64_t>(blockIdx.x) * stride + tid] = count[tid];
 }
 
-__global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a, uint64_t per_block, uint32_t stride, uint32_t bits)
+__device__ __forceinline__ void add_tile_counts(const OrderArgs& a, uint32_t stride, uint32_t* before_me, uint32_t* of_all)
 {
-    __shared__ OrderShared sh;
-    __shared__ uint32_t before_me[kMaxExperts];
-    __shared__ uint32_t of_all[kMaxExperts];
+    // The counts of all tiles, four experts a thread, the tiles shared out among groups of threads.  Every workgroup
+    // begins with its own: all of them reading the same tile at a time took 3 us longer.  Four loads at a time; a thread
+    // that has fewer tiles left reads one again.
     const uint32_t tid = threadIdx.x;
-    const uint64_t first = blockIdx.x * per_block;
-    uint64_t last = first + per_block;
-    if (last > a.slots) last = a.slots;
-    uint32_t expert[kTileR], rank[kTileR];
-    load_experts<kTileR>(a, first, expert);
-    if (tid < a.experts) {
-        before_me[tid] = 0;
-        of_all[tid] = 0;
-    }
-    rank_in_waves<kTileR>(a, sh, bits, expert, rank);
-    __syncthreads();
-    // The counts of all tiles, four experts a thread, the tiles shared out among groups of threads.  Every workgroup begins
-    // with its own: all of them reading the same tile at a time took 3 us longer.  Four loads at a time; a thread that has fewer
-    // tiles left reads one again.
     const uint32_t quads = stride / 4;
     const uint32_t groups = kThreads / quads;
     const uint32_t group = tid / quads;
@@ -268,13 +257,58 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
                 atomicAdd(&before_me[e + i], before[i]);
             }
     }
+}
+
+// DIRECT: a workgroup counts all slots itself, into kCopies counters an expert that neighbouring lanes use in turn (equal
+// experts in one instruction wait for each other).  Otherwise the counts of tiles are there from
+// route_order_count_kernel.
+template <bool DIRECT>
+__global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a, uint64_t per_block, uint32_t stride, uint32_t bits)
+{
+    constexpr uint32_t kCopies = DIRECT ? 4 : 1;
+    __shared__ OrderShared sh;
+    __shared__ uint32_t before_me[kMaxExperts * kCopies];
+    __shared__ uint32_t of_all[kMaxExperts * kCopies];  // DIRECT: of this tile and those behind
+    const uint32_t tid = threadIdx.x;
+    const uint64_t first = blockIdx.x * per_block;
+    uint64_t last = first + per_block;
+    if (last > a.slots) last = a.slots;
+    uint32_t expert[kTileR], rank[kTileR];
+    load_experts<kTileR>(a, first, expert);
+    for (uint32_t i = tid; i < a.experts * kCopies; i += kThreads) {
+        before_me[i] = 0;
+        of_all[i] = 0;
+    }
+    rank_in_waves<kTileR>(a, sh, bits, expert, rank);
+    __syncthreads();
+    if constexpr (DIRECT) {
+        for (uint64_t at = 0; at < a.slots; at += 8 * kThreads) {
+            uint32_t e[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const uint64_t slot = at + i * kThreads + tid;
+                e[i] = slot < a.slots ? static_cast<uint32_t>(a.ids[slot]) : a.experts;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                uint32_t* count = at + i * kThreads < first ? before_me : of_all;
+                if (e[i] < a.experts) atomicAdd(&count[e[i] * kCopies + tid % kCopies], 1u);
+            }
+        }
+    } else {
+        add_tile_counts(a, stride, before_me, of_all);
+    }
     __syncthreads();
     uint32_t kept = 0, taken = 0, in_tile = 0;
     if (tid < a.experts) {
         in_tile = scan_waves(sh, tid);
-        kept = of_all[tid];
+#pragma unroll
+        for (uint32_t i = 0; i < kCopies; ++i) {
+            taken += before_me[tid * kCopies + i];
+            kept += of_all[tid * kCopies + i];
+        }
+        if (DIRECT) kept += taken;
         if (kept > a.capacity) kept = a.capacity;
-        taken = before_me[tid];
         if (taken > a.capacity) taken = a.capacity;
     }
     const uint32_t padded = round_up_to(kept, a.align);
@@ -332,9 +366,14 @@ int launch_route_order(const OrderArgs& a, hipStream_t s)
     uint64_t tiles = (a.slots + kTileSlots - 1) / kTileSlots;
     const uint64_t per_block = (tiles + kRouteMaxTiles - 1) / kRouteMaxTiles * kTileSlots;
     const uint32_t blocks = static_cast<uint32_t>((a.slots + per_block - 1) / per_block);
+    if (a.slots <= kDirectSlots) {
+        hipLaunchKernelGGL(route_order_kernel<true>, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride, bits);
+        MRS_CHECK_LAUNCH("route_order_kernel");
+        return MRS_OK;
+    }
     hipLaunchKernelGGL(route_order_count_kernel, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride);
     MRS_CHECK_LAUNCH("route_order_count_kernel");
-    hipLaunchKernelGGL(route_order_kernel, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride, bits);
+    hipLaunchKernelGGL(route_order_kernel<false>, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride, bits);
     MRS_CHECK_LAUNCH("route_order_kernel");
     return MRS_OK;
 }

@@ -12,7 +12,13 @@ namespace {
 
 constexpr uint32_t kMoveThreads = 128;     // dispatch
 constexpr uint32_t kSumThreads = 1024;     // combine and its gradient: a workgroup covers whole rows
+constexpr uint32_t kShortThreads = 128;     // ... shorter than a wave's 64 vectors
 constexpr uint32_t kMaxBlocks = 1u << 20;  // more work than that is looped over
+constexpr uint32_t kPadWaves = 2048;       // waves for the rows that fill segments up, two on a SIMD
+// combine's gradient: waves share a token's pieces evenly, but where that makes fewer waves than this, as many as there are pieces
+// for: 3 tokens of 6368 f32 (25 pieces) 36 -> 8.6 us, while
+// 3000 of 1109 (5 pieces) take 19 us evenly and 23 with four waves each.
+constexpr uint64_t kFewWaves = 2048;
 // Rows that cannot stay in the 256 MiB memory-side cache until somebody reads them again are streamed past the caches.
 constexpr uint64_t kStreamBytes = 256ull << 20;
 
@@ -23,13 +29,13 @@ struct Cut {
     uint32_t vectors;      // whole 16-byte vectors of a row
     uint32_t pieces;       // of a row
     uint32_t items;        // what groups take: tokens * pieces, or tokens * token_waves
-    uint32_t token_waves;  // combine's gradient: waves that share a token's pieces evenly, a power of two
+    uint32_t token_waves;  // combine's gradient: waves that share a token's pieces, a power of two
     uint32_t blocks;       // workgroups for the items
     uint32_t pad_blocks;   // workgroups before them that zero the rows that fill segments up
-    uint32_t pad_split;    // of these, how many share an expert
+    uint32_t pad_split;    // waves that share an expert's
 };
 
-int cut_rows(const MoveArgs& a, uint32_t element_bytes, uint32_t threads, bool whole_tokens, bool pads, Cut* out)
+int cut_rows(const MoveArgs& a, uint32_t element_bytes, uint32_t threads, uint32_t short_threads, bool whole_tokens, bool pads, Cut* out)
 {
     Cut c;
     const uint64_t row_bytes = static_cast<uint64_t>(a.hidden) * element_bytes;
@@ -38,8 +44,11 @@ int cut_rows(const MoveArgs& a, uint32_t element_bytes, uint32_t threads, bool w
     c.lanes_log2 = 0;
     while (c.lanes_log2 < 6 && (1u << c.lanes_log2) < touched) ++c.lanes_log2;
     c.pieces = (touched + (1u << c.lanes_log2) - 1) >> c.lanes_log2;
+    if (c.lanes_log2 < 6) threads = short_threads;
     c.token_waves = 1;
     while (c.pieces % (c.token_waves * 2) == 0 && c.token_waves < threads / 64) c.token_waves *= 2;
+    if (a.tokens * c.token_waves < kFewWaves)
+        while (c.token_waves * 2 <= c.pieces && c.token_waves < threads / 64) c.token_waves *= 2;
     const uint64_t items = a.tokens * (whole_tokens ? c.token_waves : c.pieces);
     const uint32_t per_block = threads >> c.lanes_log2;
     uint64_t blocks = (items + per_block - 1) / per_block;
@@ -51,8 +60,10 @@ int cut_rows(const MoveArgs& a, uint32_t element_bytes, uint32_t threads, bool w
     c.pad_split = 0;
     c.pad_blocks = 0;
     if (pads && a.align > 1) {
-        c.pad_split = a.align - 1 < 8 ? a.align - 1 : 8;
-        c.pad_blocks = a.experts * c.pad_split;
+        c.pad_split = kPadWaves / a.experts;
+        if (c.pad_split > a.align - 1) c.pad_split = a.align - 1;
+        if (c.pad_split == 0) c.pad_split = 1;
+        c.pad_blocks = (a.experts * c.pad_split + threads / 64 - 1) / (threads / 64);
     }
     *out = c;
     return MRS_OK;
@@ -73,24 +84,25 @@ __device__ __forceinline__ void put(void* p, RouteVec v)
         store_vec(p, v);
 }
 
-// Zeroes the rows of one expert's segment that no slot has.
+// A wave's share of the rows of one expert's segment that no slot has: zeros.
 template <typename Elem, uint32_t THREADS>
-__device__ void zero_padding(const MoveArgs& a, const Cut& c, uint32_t block)
+__device__ void zero_padding(const MoveArgs& a, const Cut& c)
 {
-    const uint32_t e = block / c.pad_split;
-    const uint32_t part = block % c.pad_split;
+    const uint32_t item = __builtin_amdgcn_readfirstlane(blockIdx.x * (THREADS / 64) + threadIdx.x / 64);
+    const uint32_t e = item / c.pad_split;
+    if (e >= a.experts) return;
     const int64_t first = static_cast<int64_t>(a.offsets[e]) + a.counts[e];
     int64_t end = a.offsets[e + 1];
     if (end > a.rows) end = a.rows;
     if (first < 0) return;
     Elem* out = static_cast<Elem*>(a.rows_out);
     constexpr uint32_t N = 16 / sizeof(Elem);
-    const uint32_t whole = a.hidden / N;
+    const uint32_t lane = threadIdx.x & 63u;
     const RouteVec zero = {0, 0, 0, 0};
-    for (int64_t r = first + part; r < end; r += c.pad_split) {
+    for (int64_t r = first + item % c.pad_split; r < end; r += c.pad_split) {
         Elem* row = out + static_cast<uint64_t>(r) * a.ld_rows_out;
-        for (uint32_t v = threadIdx.x; v < whole; v += THREADS) store_vec(row + static_cast<uint64_t>(v) * N, zero);
-        for (uint32_t h = whole * N + threadIdx.x; h < a.hidden; h += THREADS) row[h] = Elem(0);
+        for (uint32_t v = lane; v < c.vectors; v += 64) store_vec(row + v * N, zero);
+        for (uint32_t h = c.vectors * N + lane; h < a.hidden; h += 64) row[h] = Elem(0);
     }
 }
 
@@ -137,7 +149,7 @@ __global__ __launch_bounds__(kMoveThreads) void route_dispatch_kernel(const Elem
                                                                       const Cut c)
 {
     if (blockIdx.x < c.pad_blocks) {
-        zero_padding<Elem, kMoveThreads>(a, c, blockIdx.x);
+        zero_padding<Elem, kMoveThreads>(a, c);
         return;
     }
     constexpr uint32_t N = 16 / sizeof(Elem);
@@ -174,14 +186,14 @@ __global__ __launch_bounds__(kMoveThreads) void route_dispatch_kernel(const Elem
 // workgroups of 4 waves 0.214, with ordinary loads 0.231, with neither 0.24.  Where the rows fit the memory-side
 // cache ordinary loads win: 64 MiB of them 13.5 against 14 us.
 template <typename T, uint32_t K, bool MORE, bool WEIGHTED, bool WAVE, bool STREAM>
-__global__ __launch_bounds__(kSumThreads) void route_combine_kernel(const T* __restrict__ rows, T* __restrict__ out,
+__global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_combine_kernel(const T* __restrict__ rows, T* __restrict__ out,
                                                                     const int32_t* __restrict__ row_of_slot,
                                                                     const float* __restrict__ weights, const MoveArgs a, const Cut c)
 {
-    constexpr uint32_t N = 16 / sizeof(T);
+    constexpr uint32_t N = 16 / sizeof(T), THREADS = WAVE ? kSumThreads : kShortThreads;
     const uint32_t lane = threadIdx.x & ((1u << c.lanes_log2) - 1);
-    const uint32_t step = c.blocks * (kSumThreads >> c.lanes_log2);
-    for (uint32_t item = first_item<kSumThreads, WAVE>(c); item < c.items; item += step) {
+    const uint32_t step = c.blocks * (THREADS >> c.lanes_log2);
+    for (uint32_t item = first_item<THREADS, WAVE>(c); item < c.items; item += step) {
         const uint32_t t = item / c.pieces, piece = item - t * c.pieces;
         T* to = out + static_cast<uint64_t>(t) * a.ld_token_out;
         const uint32_t v = (piece << c.lanes_log2) + lane;
@@ -262,21 +274,22 @@ __device__ __forceinline__ float sums_over_wave(const float (&v)[K])
 }
 
 template <typename T, uint32_t K, bool WAVE, bool STREAM>
-__global__ __launch_bounds__(kSumThreads) void route_combine_backward_kernel(const T* __restrict__ rows, const T* __restrict__ out_grad,
+__global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_combine_backward_kernel(const T* __restrict__ rows, const T* __restrict__ out_grad,
                                                                              T* __restrict__ rows_grad,
                                                                              const int32_t* __restrict__ row_of_slot,
                                                                              const float* __restrict__ weights, const MoveArgs a,
                                                                              const Cut c)
 {
+    constexpr uint32_t THREADS = WAVE ? kSumThreads : kShortThreads;
     if (blockIdx.x < c.pad_blocks) {
-        zero_padding<T, kSumThreads>(a, c, blockIdx.x);
+        zero_padding<T, THREADS>(a, c);
         return;
     }
     constexpr uint32_t N = 16 / sizeof(T);
-    __shared__ float partial[2][kSumThreads / 64][K];
+    __shared__ float partial[2][THREADS / 64][K];
     const uint32_t lanes = 1u << c.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const uint32_t per_block = kSumThreads >> c.lanes_log2;
-    uint32_t item = first_item<kSumThreads, WAVE>(c);
+    const uint32_t per_block = THREADS >> c.lanes_log2;
+    uint32_t item = first_item<THREADS, WAVE>(c);
     uint32_t half = 0;
     // the whole workgroup leaves together: its first item is what counts
     for (uint32_t base = (blockIdx.x - c.pad_blocks) * per_block; base < c.items; base += c.blocks * per_block, item += c.blocks * per_block) {
@@ -344,12 +357,12 @@ __global__ __launch_bounds__(kSumThreads) void route_combine_backward_kernel(con
                     half ^= 1;  // the next round writes the other half: one barrier a round is enough
                 }
             } else {
+for (uint32_t m = lanes >> 1; m > 0; m >>= 1)
 #pragma unroll
-                for (uint32_t j = 0; j < K; ++j) {
-                    float d = dot[j];
-                    for (uint32_t m = lanes >> 1; m > 0; m >>= 1) d += __shfl_xor(d, static_cast<int>(m), static_cast<int>(lanes));
-                    if (item < c.items && j0 + j < a.topk && lane == (j & (lanes - 1))) sums[j] = d;
-                }
+                    for (uint32_t j = 0; j < K; ++j) dot[j] += __shfl_xor(dot[j], static_cast<int>(m), static_cast<int>(lanes));
+#pragma unroll
+                for (uint32_t j = 0; j < K; ++j)
+                    if (item < c.items && j0 + j < a.topk && lane == (j & (lanes - 1))) sums[j] = dot[j];
             }
         }
     }
@@ -371,7 +384,7 @@ template <typename E>
 int start_dispatch(const MoveArgs& a, hipStream_t s)
 {
     Cut c;
-    if (int rc = cut_rows(a, sizeof(E), kMoveThreads, false, true, &c)) return rc;
+    if (int rc = cut_rows(a, sizeof(E), kMoveThreads, kMoveThreads, false, true, &c)) return rc;
     const dim3 grid(c.blocks + c.pad_blocks), block(kMoveThreads);
     with_slots(a.topk, [&](auto k, auto) {
         constexpr uint32_t K = decltype(k)::value;
@@ -390,8 +403,8 @@ template <typename T, bool WEIGHTED>
 int start_combine(const MoveArgs& a, hipStream_t s)
 {
     Cut c;
-    if (int rc = cut_rows(a, sizeof(T), kSumThreads, false, false, &c)) return rc;
-    const dim3 grid(c.blocks), block(kSumThreads);
+    if (int rc = cut_rows(a, sizeof(T), kSumThreads, kShortThreads, false, false, &c)) return rc;
+    const dim3 grid(c.blocks), block(c.lanes_log2 == 6 ? kSumThreads : kShortThreads);
     const bool stream = a.tokens * a.topk * a.hidden * sizeof(T) >= kStreamBytes;
     // a loop for more than eight slots costs the others 1 %
     with_slots(a.topk, [&](auto k, auto more) {
@@ -414,8 +427,8 @@ template <typename T>
 int start_combine_backward(const MoveArgs& a, hipStream_t s)
 {
     Cut c;
-    if (int rc = cut_rows(a, sizeof(T), kSumThreads, true, true, &c)) return rc;
-    const dim3 grid(c.blocks + c.pad_blocks), block(kSumThreads);
+    if (int rc = cut_rows(a, sizeof(T), kSumThreads, kShortThreads, true, true, &c)) return rc;
+    const dim3 grid(c.blocks + c.pad_blocks), block(c.lanes_log2 == 6 ? kSumThreads : kShortThreads);
     const bool stream = 2 * a.tokens * a.topk * a.hidden * sizeof(T) >= kStreamBytes;  // read and written
     with_slots(a.topk, [&](auto k, auto) {
         constexpr uint32_t K = decltype(k)::value;

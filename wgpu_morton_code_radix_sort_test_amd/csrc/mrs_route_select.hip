@@ -448,7 +448,14 @@ void choose(const SelectArgs& a, hipStream_t s)
         else
             start<T, 32, 32, true>(a, s);
     } else if (a.experts <= 256 && a.topk <= 16) {  // a lane for every slot
-        start<T, 16, 16, false>(a, s);
+        if (a.experts <= 16)
+            start<T, 16, 1, false>(a, s);
+        else if (a.experts <= 64)
+            start<T, 16, 4, false>(a, s);
+        else if (a.experts <= 128)
+            start<T, 16, 8, false>(a, s);
+        else
+            start<T, 16, 16, false>(a, s);
     } else if (a.experts <= 512) {
         start<T, 32, 16, false>(a, s);
     } else {
