@@ -210,7 +210,7 @@ def test_order(ctx, mrs, tokens, experts, topk, align, capacity):
     check_order(mrs, ctx, ids, experts, align, capacity, extra=3)
 
 
-@pytest.mark.parametrize("slots", [64, 65, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 12288])
+@pytest.mark.parametrize("slots", [64, 65, 1024, 1025, 2048, 2049, 4096, 4097, 8193, 16384, 49151, 49152, 49153, 53248, 53249])
 def test_order_around_tile_sizes(ctx, mrs, slots):
     g = torch.Generator().manual_seed(slots)
     ids = (torch.randn(slots, 1, generator=g) * 3 + 8).to(torch.int32)  # crowded in the middle, some outside
@@ -218,7 +218,7 @@ def test_order_around_tile_sizes(ctx, mrs, slots):
         check_order(mrs, ctx, ids, 16, align, capacity, extra=1)
 
 
-@pytest.mark.parametrize("tokens", [700, 9000])
+@pytest.mark.parametrize("tokens", [400, 9000, 30000])
 def test_order_of_odd_ids(ctx, mrs, tokens):
     """One expert has everything; nobody has anything; runs; numbers far outside; one expert after the other."""
     topk, experts = 2, 37

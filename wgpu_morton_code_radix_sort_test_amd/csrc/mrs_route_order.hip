@@ -7,13 +7,14 @@
 // the equal lanes below; a scan over the waves' counters gives the rank inside the tile.  No
 // atomics decide an order, so rows are the same every time.
 //
-// Up to kSmallSlots slots one workgroup does everything in one launch (256 experts: 4.0 us for 512 slots, 7.3 for 4096;
-// 8192 took 11.3); what bounds it is the launch and the chain of LDS accesses and barriers.  Up to kDirectSlots one launch
-// of several workgroups, each of which counts all slots by itself (16384 slots 9.2 us, with two launches 10.5; 65536 14.2
-// and 11.0).  Above, a first launch counts tiles, and in a second one every workgroup adds up the counts of the tiles
-// before its own by itself (at most 256 tiles of `experts` counts, read from L2) instead of waiting for a scan launch
-// between the two.  2^20 slots, 256 experts: 17 us, 4 of them for the counts, about 3 each for adding them up and for the
-// writes to slot_of_row in runs of some 16 rows.
+// Up to kSmallSlots slots one workgroup does everything (512 slots, 256 experts: 4.0 us); what bounds it is the launch and
+// the chain of LDS accesses and barriers.  Up to kDirectSlots one launch of several workgroups, a slot a thread, each of
+// which counts all slots by itself (4096 slots 5.3 us, 16384 6.3, 32768 8.0; four slots a thread 9.2 and 10.7 for the
+// latter, one workgroup 7.3 for 4096).  Above, a first launch counts tiles, and in a second one every workgroup adds up
+// the counts of the tiles before its own by itself (at most 256 tiles of `experts` counts, read from L2) instead of
+// waiting for a scan launch between the two (32768 slots 10.7 us, 65536 11.0, where the direct form takes 11.5).  2^20
+// slots: 17 us, 4 of them for the counts, about 3 each for adding them up and for the writes to slot_of_row in runs of
+// some 16 rows.
 #include "mrs_route.hpp"
 
 namespace mrs {
@@ -24,10 +25,9 @@ constexpr uint32_t kWaves = 16;
 constexpr uint32_t kThreads = kWaves * 64;
 constexpr uint32_t kMaxExperts = MRS_ROUTE_MAX_EXPERTS;
 static_assert(kMaxExperts <= kThreads, "one thread per expert in the scans");
-constexpr uint32_t kSmallSlots = kThreads * 4;
-constexpr uint32_t kDirectSlots = 16384;
-constexpr uint32_t kTileR = 4;
-constexpr uint32_t kTileSlots = kThreads * kTileR;
+constexpr uint32_t kSmallSlots = kThreads;
+constexpr uint32_t kDirectSlots = 49152;
+constexpr uint32_t kTileSlots = kThreads * 4;
 
 struct OrderShared {
     alignas(4) uint16_t wave_count[kWaves][kMaxExperts];  // slots per wave, then those of the waves before
@@ -169,15 +169,14 @@ __device__ __forceinline__ void mark_empty_rows(const OrderArgs& a, const OrderS
         a.slot_of_row[r] = -1;
 }
 
-// R slots a thread, all in one workgroup.
-template <uint32_t R>
+// A slot a thread, all in one workgroup.
 __global__ __launch_bounds__(kThreads) void route_order_small_kernel(const OrderArgs a, uint32_t bits)
 {
     __shared__ OrderShared sh;
     const uint32_t tid = threadIdx.x;
-    uint32_t expert[R], rank[R];
-    load_experts<R>(a, 0, expert);
-    rank_in_waves<R>(a, sh, bits, expert, rank);
+    uint32_t expert[1], rank[1];
+    load_experts<1>(a, 0, expert);
+    rank_in_waves<1>(a, sh, bits, expert, rank);
     __syncthreads();
     uint32_t kept = 0;
     if (tid < a.experts) {
@@ -197,7 +196,7 @@ __global__ __launch_bounds__(kThreads) void route_order_small_kernel(const Order
         if (tid == a.experts - 1) a.offsets[a.experts] = static_cast<int32_t>(end);
     }
     __syncthreads();
-    write_rows<R>(a, sh, 0, expert, rank);
+    write_rows<1>(a, sh, 0, expert, rank);
     mark_empty_rows(a, sh, end, 0, 1);
 }
 
@@ -266,6 +265,7 @@ template <bool DIRECT>
 __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a, uint64_t per_block, uint32_t stride, uint32_t bits)
 {
     constexpr uint32_t kCopies = DIRECT ? 4 : 1;
+    constexpr uint32_t R = DIRECT ? 1 : kTileSlots / kThreads;
     __shared__ OrderShared sh;
     __shared__ uint32_t before_me[kMaxExperts * kCopies];
     __shared__ uint32_t of_all[kMaxExperts * kCopies];  // DIRECT: of this tile and those behind
@@ -273,13 +273,13 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
     const uint64_t first = blockIdx.x * per_block;
     uint64_t last = first + per_block;
     if (last > a.slots) last = a.slots;
-    uint32_t expert[kTileR], rank[kTileR];
-    load_experts<kTileR>(a, first, expert);
+    uint32_t expert[R], rank[R];
+    load_experts<R>(a, first, expert);
     for (uint32_t i = tid; i < a.experts * kCopies; i += kThreads) {
         before_me[i] = 0;
         of_all[i] = 0;
     }
-    rank_in_waves<kTileR>(a, sh, bits, expert, rank);
+    rank_in_waves<R>(a, sh, bits, expert, rank);
     __syncthreads();
     if constexpr (DIRECT) {
         for (uint64_t at = 0; at < a.slots; at += 8 * kThreads) {
@@ -327,10 +327,10 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
     }
     __syncthreads();
     for (uint64_t at = first;;) {
-        write_rows<kTileR>(a, sh, at, expert, rank);
-        at += kTileSlots;
+        write_rows<R>(a, sh, at, expert, rank);
+        at += kThreads * R;
         if (at >= last) break;
-        load_experts<kTileR>(a, at, expert);
+        load_experts<R>(a, at, expert);
         __syncthreads();
         if (tid < a.experts) {
             const uint32_t room = sh.room[tid];
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a
             sh.row[tid] += took;
             sh.room[tid] = room - took;
         }
-        rank_in_waves<kTileR>(a, sh, bits, expert, rank);
+        rank_in_waves<R>(a, sh, bits, expert, rank);
         __syncthreads();
         if (tid < a.experts) in_tile = scan_waves(sh, tid);
         __syncthreads();
@@ -353,24 +353,20 @@ int launch_route_order(const OrderArgs& a, hipStream_t s)
     uint32_t bits = 0;
     while ((a.experts >> bits) != 0) ++bits;  // the values 0 .. experts
     if (a.slots <= kSmallSlots) {
-        if (a.slots <= kThreads)
-            hipLaunchKernelGGL(route_order_small_kernel<1>, dim3(1), dim3(kThreads), 0, s, a, bits);
-        else if (a.slots <= 2 * kThreads)
-            hipLaunchKernelGGL(route_order_small_kernel<2>, dim3(1), dim3(kThreads), 0, s, a, bits);
-        else
-            hipLaunchKernelGGL(route_order_small_kernel<4>, dim3(1), dim3(kThreads), 0, s, a, bits);
+        hipLaunchKernelGGL(route_order_small_kernel, dim3(1), dim3(kThreads), 0, s, a, bits);
         MRS_CHECK_LAUNCH("route_order_small_kernel");
         return MRS_OK;
     }
     const uint32_t stride = (a.experts + 3) / 4 * 4;
-    uint64_t tiles = (a.slots + kTileSlots - 1) / kTileSlots;
-    const uint64_t per_block = (tiles + kRouteMaxTiles - 1) / kRouteMaxTiles * kTileSlots;
-    const uint32_t blocks = static_cast<uint32_t>((a.slots + per_block - 1) / per_block);
     if (a.slots <= kDirectSlots) {
-        hipLaunchKernelGGL(route_order_kernel<true>, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride, bits);
+        const uint32_t blocks = (static_cast<uint32_t>(a.slots) + kThreads - 1) / kThreads;
+        hipLaunchKernelGGL(route_order_kernel<true>, dim3(blocks), dim3(kThreads), 0, s, a, static_cast<uint64_t>(kThreads), stride, bits);
         MRS_CHECK_LAUNCH("route_order_kernel");
         return MRS_OK;
     }
+    const uint64_t tiles = (a.slots + kTileSlots - 1) / kTileSlots;
+    const uint64_t per_block = (tiles + kRouteMaxTiles - 1) / kRouteMaxTiles * kTileSlots;
+    const uint32_t blocks = static_cast<uint32_t>((a.slots + per_block - 1) / per_block);
     hipLaunchKernelGGL(route_order_count_kernel, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride);
     MRS_CHECK_LAUNCH("route_order_count_kernel");
     hipLaunchKernelGGL(route_order_kernel<false>, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride, bits);
