@@ -210,7 +210,7 @@ def test_order(ctx, mrs, tokens, experts, topk, align, capacity):
     check_order(mrs, ctx, ids, experts, align, capacity, extra=3)
 
 
-@pytest.mark.parametrize("slots", [64, 65, 1024, 1025, 2048, 2049, 4096, 4097, 8193, 16384, 49151, 49152, 49153, 53248, 53249])
+@pytest.mark.parametrize("slots", [64, 65, 1024, 1025, 2048, 2049, 4096, 4097, 8193, 16384, 24576, 24577, 65536, 262144, 262145])
 def test_order_around_tile_sizes(ctx, mrs, slots):
     g = torch.Generator().manual_seed(slots)
     ids = (torch.randn(slots, 1, generator=g) * 3 + 8).to(torch.int32)  # crowded in the middle, some outside
@@ -230,7 +230,7 @@ def test_order_of_odd_ids(ctx, mrs, tokens):
             check_order(mrs, ctx, flat.to(torch.int32).reshape(tokens, topk), experts, 8, capacity)
 
 
-@pytest.mark.parametrize("slots,experts", [((1 << 20) + 1, 64), (2500000, 257), (1400000, 1024)])
+@pytest.mark.parametrize("slots,experts", [((1 << 20) + 1, 64), (2500000, 257), (1400000, 1024), (65537, 1024), (140000, 1024), (300001, 300), (524289, 8)])
 def test_order_of_many_slots(ctx, mrs, slots, experts):
     """More slots than workgroups have tiles: each walks several, and an expert's capacity ends inside one."""
     g = torch.Generator().manual_seed(7)

@@ -9,12 +9,13 @@
 //
 // Up to kSmallSlots slots one workgroup does everything (512 slots, 256 experts: 4.0 us); what bounds it is the launch and
 // the chain of LDS accesses and barriers.  Up to kDirectSlots one launch of several workgroups, a slot a thread, each of
-// which counts all slots by itself (4096 slots 5.3 us, 16384 6.3, 32768 8.0; four slots a thread 9.2 and 10.7 for the
-// latter, one workgroup 7.3 for 4096).  Above, a first launch counts tiles, and in a second one every workgroup adds up
-// the counts of the tiles before its own by itself (at most 256 tiles of `experts` counts, read from L2) instead of
-// waiting for a scan launch between the two (32768 slots 10.7 us, 65536 11.0, where the direct form takes 11.5).  2^20
-// slots: 17 us, 4 of them for the counts, about 3 each for adding them up and for the writes to slot_of_row in runs of
-// some 16 rows.
+// which counts all slots by itself (4096 slots 5.3 us, 16384 6.3, 32768 8.0, where two launches take 7.3, 7.9 and 7.9;
+// one workgroup alone 7.3 for 4096).  Above, a first launch counts tiles of 1, 2 or 4 slots a thread, and in a second one
+// every workgroup adds up the counts of the tiles before its own by itself (read from L2) instead of waiting for a scan
+// launch between the two (65536 slots 7.9 us, with four slots a thread 11.0).  2^20 slots: 17 us, 4 of them for the counts,
+// about 3 each for adding them up and for the writes to slot_of_row in runs of some 16 rows.
+#include <algorithm>
+
 #include "mrs_route.hpp"
 
 namespace mrs {
@@ -26,8 +27,7 @@ constexpr uint32_t kThreads = kWaves * 64;
 constexpr uint32_t kMaxExperts = MRS_ROUTE_MAX_EXPERTS;
 static_assert(kMaxExperts <= kThreads, "one thread per expert in the scans");
 constexpr uint32_t kSmallSlots = kThreads;
-constexpr uint32_t kDirectSlots = 49152;
-constexpr uint32_t kTileSlots = kThreads * 4;
+constexpr uint32_t kDirectSlots = 24576;
 
 struct OrderShared {
     alignas(4) uint16_t wave_count[kWaves][kMaxExperts];  // slots per wave, then those of the waves before
@@ -261,11 +261,10 @@ __device__ __forceinline__ void add_tile_counts(const OrderArgs& a, uint32_t str
 // DIRECT: a workgroup counts all slots itself, into kCopies counters an expert that neighbouring lanes use in turn (equal
 // experts in one instruction wait for each other).  Otherwise the counts of tiles are there from
 // route_order_count_kernel.
-template <bool DIRECT>
+template <bool DIRECT, uint32_t R>
 __global__ __launch_bounds__(kThreads) void route_order_kernel(const OrderArgs a, uint64_t per_block, uint32_t stride, uint32_t bits)
 {
     constexpr uint32_t kCopies = DIRECT ? 4 : 1;
-    constexpr uint32_t R = DIRECT ? 1 : kTileSlots / kThreads;
     __shared__ OrderShared sh;
     __shared__ uint32_t before_me[kMaxExperts * kCopies];
     __shared__ uint32_t of_all[kMaxExperts * kCopies];  // DIRECT: of this tile and those behind
@@ -360,16 +359,25 @@ int launch_route_order(const OrderArgs& a, hipStream_t s)
     const uint32_t stride = (a.experts + 3) / 4 * 4;
     if (a.slots <= kDirectSlots) {
         const uint32_t blocks = (static_cast<uint32_t>(a.slots) + kThreads - 1) / kThreads;
-        hipLaunchKernelGGL(route_order_kernel<true>, dim3(blocks), dim3(kThreads), 0, s, a, static_cast<uint64_t>(kThreads), stride, bits);
+        hipLaunchKernelGGL((route_order_kernel<true, 1>), dim3(blocks), dim3(kThreads), 0, s, a, static_cast<uint64_t>(kThreads), stride, bits);
         MRS_CHECK_LAUNCH("route_order_kernel");
         return MRS_OK;
     }
-    const uint64_t tiles = (a.slots + kTileSlots - 1) / kTileSlots;
-    const uint64_t per_block = (tiles + kRouteMaxTiles - 1) / kRouteMaxTiles * kTileSlots;
-    const uint32_t blocks = static_cast<uint32_t>((a.slots + per_block - 1) / per_block);
-    hipLaunchKernelGGL(route_order_count_kernel, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride);
+    // Small tiles are ranked sooner, but every workgroup reads the counts of all of them: no more than 2^16 numbers, if that
+    // leaves 64 tiles (2^18 slots, 1024 experts: 256 tiles 20.7 us, 64 tiles 15.1).
+    const uint64_t most = std::max(64u, std::min(kRouteMaxTiles, 65536u / a.experts));
+    const uint32_t r = a.slots <= most * kThreads ? 1 : a.slots <= most * kThreads * 2 ? 2 : 4;
+    const uint64_t tile = static_cast<uint64_t>(kThreads) * r;
+    const uint64_t per_block = ((a.slots + tile - 1) / tile + kRouteMaxTiles - 1) / kRouteMaxTiles * tile;
+    const dim3 grid(static_cast<uint32_t>((a.slots + per_block - 1) / per_block)), block(kThreads);
+    hipLaunchKernelGGL(route_order_count_kernel, grid, block, 0, s, a, per_block, stride);
     MRS_CHECK_LAUNCH("route_order_count_kernel");
-    hipLaunchKernelGGL(route_order_kernel<false>, dim3(blocks), dim3(kThreads), 0, s, a, per_block, stride, bits);
+    if (r == 1)
+        hipLaunchKernelGGL((route_order_kernel<false, 1>), grid, block, 0, s, a, per_block, stride, bits);
+    else if (r == 2)
+        hipLaunchKernelGGL((route_order_kernel<false, 2>), grid, block, 0, s, a, per_block, stride, bits);
+    else
+        hipLaunchKernelGGL((route_order_kernel<false, 4>), grid, block, 0, s, a, per_block, stride, bits);
     MRS_CHECK_LAUNCH("route_order_kernel");
     return MRS_OK;
 }
