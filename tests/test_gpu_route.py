@@ -366,6 +366,26 @@ def test_combine_backward(ctx, mrs, tokens, experts, topk, hidden, align, dtype,
     plan.close()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("hidden", [9, 21, 300, 1109])
+def test_columns_a_kernel_visits_twice_count_once(ctx, mrs, dtype, hidden):
+    """Rows that no whole number of 16-byte vectors covers: an infinite element near the end makes its weight's gradient
+    infinite, not NaN, and comes through combine as it is."""
+    plan, route, rows, g = make_route(mrs, ctx, 4, 4, 2, drop=0.0)
+    x, dout = torch.rand(rows, hidden, generator=g).to(dtype) + 0.5, torch.rand(4, hidden, generator=g).to(dtype) + 0.5
+    for back in (1, 2, 3, min(8, hidden)):
+        y = x.clone()
+        y[:, hidden - back] = INF
+        row_of_slot = route.row_of_slot.cpu()
+        w = torch.ones(4, 2, device=ctx.device)
+        _, dw = plan.combine_backward(dout.to(ctx.device), y.to(ctx.device), route, w)
+        assert bool((dw.cpu()[row_of_slot >= 0] == INF).all())
+        out = plan.combine(y.to(ctx.device), route, w).cpu()
+        some = (row_of_slot >= 0).any(1)
+        assert bool((out[some][:, hidden - back] == INF).all())
+        assert int(torch.isinf(out).sum()) == int(some.sum())
+
+
 def test_rows_past_4_gib(ctx, mrs):
     """Row offsets beyond 32 bits: rows 2 x 65792 bytes apart, 40000 of them."""
     tokens, experts, topk, hidden, stride = 10000, 16, 4, 72, 65792

@@ -23,10 +23,13 @@ constexpr uint64_t kFewWaves = 2048;
 constexpr uint64_t kStreamBytes = 256ull << 20;
 
 // How a launch cuts its work.  A group of lanes -- a power of two up to a wave's 64, enough for the row if they can be --
-// takes a piece of a row, a 16-byte vector a lane.
+// takes a piece of a row, a 16-byte vector a lane.  Where the last vector would reach behind the row it ends with it instead and
+// repeats some columns of the one before: they are worked out alike and written twice.  Only rows shorter than a
+// vector go element by element.
 struct Cut {
     uint32_t lanes_log2;
-    uint32_t vectors;      // whole 16-byte vectors of a row
+    uint32_t vectors;      // 16-byte vectors of a row, 0 if it is shorter than one
+    uint32_t last_column;  // where the last vector starts
     uint32_t pieces;       // of a row
     uint32_t items;        // what groups take: tokens * pieces, or tokens * token_waves
     uint32_t token_waves;  // combine's gradient: waves that share a token's pieces, a power of two
@@ -39,8 +42,9 @@ int cut_rows(const MoveArgs& a, uint32_t element_bytes, uint32_t threads, uint32
 {
     Cut c;
     const uint64_t row_bytes = static_cast<uint64_t>(a.hidden) * element_bytes;
-    c.vectors = static_cast<uint32_t>(row_bytes / 16);
     const uint32_t touched = static_cast<uint32_t>((row_bytes + 15) / 16);
+    c.vectors = row_bytes < 16 ? 0 : touched;
+    c.last_column = row_bytes < 16 ? 0 : a.hidden - 16 / element_bytes;
     c.lanes_log2 = 0;
     while (c.lanes_log2 < 6 && (1u << c.lanes_log2) < touched) ++c.lanes_log2;
     c.pieces = (touched + (1u << c.lanes_log2) - 1) >> c.lanes_log2;
@@ -101,8 +105,8 @@ __device__ void zero_padding(const MoveArgs& a, const Cut& c)
     const RouteVec zero = {0, 0, 0, 0};
     for (int64_t r = first + item % c.pad_split; r < end; r += c.pad_split) {
         Elem* row = out + static_cast<uint64_t>(r) * a.ld_rows_out;
-        for (uint32_t v = lane; v < c.vectors; v += 64) store_vec(row + v * N, zero);
-        for (uint32_t h = c.vectors * N + lane; h < a.hidden; h += 64) row[h] = Elem(0);
+        for (uint32_t v = lane; v < c.vectors; v += 64) store_vec(row + min(v * N, c.last_column), zero);
+        if (c.vectors == 0 && lane < a.hidden) row[lane] = Elem(0);
     }
 }
 
@@ -159,17 +163,18 @@ __global__ __launch_bounds__(kMoveThreads) void route_dispatch_kernel(const Elem
         const uint32_t t = item / c.pieces, piece = item - t * c.pieces;
         const Elem* in = x + static_cast<uint64_t>(t) * a.ld_token_in;
         const uint32_t v = (piece << c.lanes_log2) + lane;
+        const uint32_t column = min(v * N, c.last_column);
         RouteVec d = {0, 0, 0, 0};
-        if (v < c.vectors) d = load_vec(in + v * N);
+        if (v < c.vectors) d = load_vec(in + column);
         for (uint32_t j0 = 0; j0 < a.topk; j0 += K) {
             uint32_t r[K];
             load_slots<K>(row_of_slot, t, j0, a, r);
             if (v < c.vectors) {
 #pragma unroll
                 for (uint32_t j = 0; j < K; ++j)
-                    if (r[j] < a.rows) store_vec(out + r[j] * a.ld_rows_out + v * N, d);
+                    if (r[j] < a.rows) store_vec(out + r[j] * a.ld_rows_out + column, d);
             }
-            for (uint32_t h = c.vectors * N + lane; piece == c.pieces - 1 && h < a.hidden; h += 1u << c.lanes_log2) {
+            for (uint32_t h = lane; c.vectors == 0 && h < a.hidden; h += 1u << c.lanes_log2) {
                 const Elem e = in[h];
 #pragma unroll
                 for (uint32_t j = 0; j < K; ++j)
@@ -197,6 +202,7 @@ __global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_comb
         const uint32_t t = item / c.pieces, piece = item - t * c.pieces;
         T* to = out + static_cast<uint64_t>(t) * a.ld_token_out;
         const uint32_t v = (piece << c.lanes_log2) + lane;
+        const uint32_t column = min(v * N, c.last_column);
         uint32_t r[K];
         float w[K];
         load_slots<K>(row_of_slot, t, 0, a, r);
@@ -210,7 +216,7 @@ __global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_comb
 #pragma unroll
                 for (uint32_t j = 0; j < K; ++j) {
                     d[j] = RouteVec{0, 0, 0, 0};
-                    if (r[j] < a.rows) d[j] = get<STREAM>(rows + r[j] * a.ld_rows_in + v * N);
+                    if (r[j] < a.rows) d[j] = get<STREAM>(rows + r[j] * a.ld_rows_in + column);
                 }
 #pragma unroll
                 for (uint32_t j = 0; j < K; ++j) {
@@ -227,9 +233,9 @@ __global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_comb
             RouteElems<T> o;
 #pragma unroll
             for (uint32_t i = 0; i < N; ++i) o.e[i] = static_cast<T>(acc[i]);
-            put<STREAM>(to + v * N, as_vec(o));
+            put<STREAM>(to + column, as_vec(o));
         }
-        for (uint32_t h = c.vectors * N + lane; piece == c.pieces - 1 && h < a.hidden; h += 1u << c.lanes_log2) {
+        for (uint32_t h = lane; c.vectors == 0 && h < a.hidden; h += 1u << c.lanes_log2) {
             float acc = 0.0f;
             for (uint32_t j = 0; j < a.topk; ++j) {
                 uint32_t r[1];
@@ -304,13 +310,17 @@ __global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_comb
                 load_slots<K>(row_of_slot, t, j0, a, r);
                 load_weights<K>(weights, t, j0, a, w);
                 const T* grad = out_grad + static_cast<uint64_t>(t) * a.ld_token_in;
-                for (uint32_t v = (share << c.lanes_log2) + lane; v < c.vectors; v += c.token_waves << c.lanes_log2) {
-                    const RouteElems<T> ge = as_elems<T>(get<STREAM>(grad + v * N));
+                // LAST: the piece holds a vector that repeats columns of the one before; they count once
+                const auto walk = [&](uint32_t v, auto last) {
+                    constexpr bool LAST = decltype(last)::value;
+                    const uint32_t column = LAST ? min(v * N, c.last_column) : v * N;
+                    const uint32_t repeated = LAST ? v * N - column : 0;
+                    const RouteElems<T> ge = as_elems<T>(get<STREAM>(grad + column));
                     RouteVec d[K];
 #pragma unroll
                     for (uint32_t j = 0; j < K; ++j) {
                         d[j] = RouteVec{0, 0, 0, 0};
-                        if (r[j] < a.rows) d[j] = get<STREAM>(rows + r[j] * a.ld_rows_in + v * N);
+                        if (r[j] < a.rows) d[j] = get<STREAM>(rows + r[j] * a.ld_rows_in + column);
                     }
 #pragma unroll
                     for (uint32_t j = 0; j < K; ++j) {
@@ -320,13 +330,20 @@ __global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_comb
 #pragma unroll
                         for (uint32_t i = 0; i < N; ++i) {
                             const float g = to_f32(ge.e[i]);
-                            dot[j] = fmaf(g, to_f32(e.e[i]), dot[j]);
+                            const float sum = fmaf(g, to_f32(e.e[i]), dot[j]);
+                            dot[j] = LAST && i < repeated ? dot[j] : sum;
                             o.e[i] = static_cast<T>(w[j] * g);
                         }
-                        put<STREAM>(rows_grad + r[j] * a.ld_rows_out + v * N, as_vec(o));
+                        put<STREAM>(rows_grad + r[j] * a.ld_rows_out + column, as_vec(o));
                     }
+                };
+                for (uint32_t v = (share << c.lanes_log2) + lane; v < c.vectors; v += c.token_waves << c.lanes_log2) {
+                    if ((v - lane + lanes) * N > a.hidden)
+                        walk(v, std::true_type{});
+                    else
+                        walk(v, std::false_type{});
                 }
-                for (uint32_t h = c.vectors * N + lane; share == c.token_waves - 1 && h < a.hidden; h += lanes) {
+                for (uint32_t h = lane; c.vectors == 0 && h < a.hidden; h += lanes) {
                     const float g = to_f32(grad[h]);
 #pragma unroll
                     for (uint32_t j = 0; j < K; ++j) {
