@@ -529,6 +529,42 @@ def test_calls_replay_from_a_graph(ctx, mrs):
             assert torch.equal(got, want)
 
 
+def test_two_graphs_of_one_plan_and_two_plans_at_once(ctx, mrs):
+    """Graphs that share a plan's memory, replayed one after the other; then plans of their own on streams of their own."""
+    dev, n, experts = ctx.device, 120000, 50
+    g = torch.Generator().manual_seed(12)
+    ids = [torch.randint(-1, experts, (n, 1), generator=g, dtype=torch.int32) for _ in range(4)]
+    want = [ref.order(i, experts, 8, 0, n + 7 * experts)[0] for i in ids]
+    plan = mrs.RoutePlan(ctx, n, experts, 1, align=8)
+    buffers, graphs, maps = [], [], []
+    side = torch.cuda.Stream()
+    for k in range(2):
+        buffers.append(ids[k].to(dev))
+        maps.append(plan.order(buffers[k]))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            plan.order(buffers[k], maps[k])
+        graphs.append(graph)
+    for k, new in ((0, 0), (1, 1), (0, 2), (1, 3), (0, 1), (1, 0)):
+        buffers[k].copy_(ids[new].to(dev))
+        graphs[k].replay()
+        graphs[1 - k].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(maps[k].row_of_slot.cpu(), want[new])
+    plans = [plan, mrs.RoutePlan(ctx, n, experts, 1, align=8)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    on_dev = [i.to(dev) for i in ids]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for k in range(2):
+            plans[k].order(on_dev[k + 2], maps[k], stream=streams[k])
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert torch.equal(maps[k].row_of_slot.cpu(), want[k + 2])
+    del graphs
+
+
 def test_calls_take_the_stream_they_are_given(ctx, mrs):
     """Behind slow work on another stream: a call that ran elsewhere would read the old contents."""
     dev = ctx.device
