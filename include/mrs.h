@@ -566,7 +566,8 @@ typedef struct mrs_route_map {
 int mrs_route_create(mrs_context* ctx, const mrs_route_desc* desc, mrs_route** out);
 int mrs_route_destroy(mrs_route* route);
 /* Host only: the most rows the slots of `desc` can take,
- * n + min(n, experts) * (align - 1) for n = tokens * topk, or what `capacity` limits it to. */
+ * n + min(n, experts) * (align - 1) for n = tokens * topk, or what `capacity` limits it to.  More for
+ * more tokens, never less: buffers of this size serve any call of up to `tokens` tokens. */
 int mrs_route_max_rows(const mrs_route_desc* desc, uint64_t* rows);
 /* ids[t, :] = the topk largest keys of row t in descending order, equal keys lowest expert first, where
  * key[e] = f32(scores[t, e]) + bias[e] (one addition in 32 bits; bias may be NULL).  An expert takes

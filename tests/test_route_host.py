@@ -52,6 +52,21 @@ def test_max_rows_holds_the_fullest_ordering():
         assert int(offsets[-1]) <= rows
 
 
+def test_max_rows_never_falls_as_tokens_grow():
+    """A plan's buffers hold the ordering of any smaller call."""
+    g = torch.Generator().manual_seed(4)
+    shapes = [(8, 2, 64, 64), (64, 8, 128, 128), (8, 2, 128, 128), (64, 1, 128, 100), (1024, 32, 1024, 1), (3, 1, 7, (1 << 64) - 1)]
+    for _ in range(60):
+        experts, topk, align = (int(torch.randint(1, hi, (1,), generator=g)) for hi in (65, 9, 130))
+        shapes.append((experts, topk, align, int(torch.randint(1, 200, (1,), generator=g))))
+    for experts, topk, align, capacity in shapes:
+        before = 0
+        for tokens in range(0, 300):
+            rc, rows = _max_rows(tokens=tokens, experts=experts, topk=topk, align=align, capacity=capacity)
+            assert rc == _lib.MRS_OK and rows >= before, (experts, topk, align, capacity, tokens)
+            before = rows
+
+
 @pytest.mark.parametrize("kw,word", [
     (dict(experts=0), "experts"), (dict(experts=1025), "experts"), (dict(topk=0), "topk"), (dict(topk=33), "topk"),
     (dict(align=0), "align"), (dict(align=1025), "align"), (dict(gate=2), "gate"), (dict(normalize=2), "normalize"),

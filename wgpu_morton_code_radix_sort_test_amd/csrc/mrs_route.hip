@@ -19,7 +19,9 @@ uint64_t max_rows_of(const mrs_route_desc& d, uint64_t tokens)
     const uint64_t n = tokens * static_cast<uint64_t>(d.topk);
     const uint64_t experts = static_cast<uint64_t>(d.experts), align = static_cast<uint64_t>(d.align);
     const uint64_t rows = n + (n < experts ? n : experts) * (align - 1);
-    if (d.capacity == 0 || d.capacity >= n) return rows;
+    // Both bounds hold for any n and neither falls as n grows, so nor does their minimum: buffers for `tokens` tokens hold
+    // fewer as well.  A capacity of 2^31 limits nothing and would overflow the product.
+    if (d.capacity == 0 || d.capacity > kMaxRows) return rows;
     const uint64_t limited = experts * ((d.capacity + align - 1) / align * align);
     return limited < rows ? limited : rows;
 }
