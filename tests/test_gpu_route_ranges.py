@@ -3,6 +3,7 @@ than one grid takes, offsets past 4 GiB."""
 import pytest
 import torch
 
+import route_ref as ref
 from test_gpu_route import check_order, mrs  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -18,3 +19,49 @@ def test_order_with_a_capacity_and_fewer_tokens_than_the_plan(ctx, mrs, tokens, 
         check_order(mrs, ctx, ids, experts, align, capacity, plan=plan)
         assert plan.order(ids.to(ctx.device)).slot_of_row.numel() == plan.max_rows
         check_order(mrs, ctx, torch.zeros_like(ids), experts, align, capacity, plan=plan)  # all in one segment
+
+
+def test_one_map_for_batches_of_different_sizes(ctx, mrs):
+    """Forward and backward of a large batch, then of smaller and larger ones, through the same map and buffers.  Rows are copies of
+    x, so the gradient of x is the sum of a token's topk rows of the gradient: small whole numbers, exact."""
+    dev, experts, topk, hidden = ctx.device, 16, 3, 40
+    plan = mrs.RoutePlan(ctx, 500, experts, topk, align=4)
+    route = plan.new_map()
+    g = torch.Generator().manual_seed(5)
+    for tokens in (500, 7, 90, 1, 500):
+        ids = torch.randint(-1, experts, (tokens, topk), generator=g, dtype=torch.int32)
+        assert plan.order(ids.to(dev), route) is route and route.tokens == tokens
+        grad = torch.randint(-8, 9, (plan.max_rows, hidden), generator=g).float()
+        got = plan.dispatch_backward(grad.to(dev), route)
+        row_of_slot = ref.order(ids, experts, 4, 0, plan.max_rows)[0].long()
+        want = (grad[row_of_slot.clamp(min=0)] * (row_of_slot >= 0).unsqueeze(2)).sum(1)
+        assert torch.equal(got.cpu(), want)
+        assert torch.equal(plan.dispatch_backward(grad.to(dev), route, tokens=tokens).cpu(), want)
+
+
+def test_a_map_that_a_graph_writes_too(ctx, mrs):
+    """Replays say nothing to the host: where their number of tokens is not the last eager call's, it has to be given."""
+    dev, experts, hidden = ctx.device, 8, 24
+    plan = mrs.RoutePlan(ctx, 300, experts, 2)
+    route = plan.new_map()
+    g = torch.Generator().manual_seed(6)
+    ids = torch.randint(0, experts, (300, 2), generator=g, dtype=torch.int32).to(dev)
+    grad = torch.randint(-8, 9, (plan.max_rows, hidden), generator=g).float().to(dev)
+    few = ids[:50].contiguous()
+    plan.order(few, route)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.order(few, route)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        got = plan.dispatch_backward(grad, route)
+        assert torch.equal(got, plan.dispatch_backward(grad, plan.order(few)))
+    plan.order(ids, route)
+    with pytest.raises(ValueError, match="tokens"):
+        plan.dispatch_backward(grad, route)
+    whole = plan.dispatch_backward(grad, route, tokens=300)
+    assert torch.equal(whole, plan.dispatch_backward(grad, plan.order(ids)))
+    graph.replay()
+    assert torch.equal(plan.dispatch_backward(grad, route, tokens=50), got)

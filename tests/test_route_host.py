@@ -148,6 +148,66 @@ def test_tensor_checks(monkeypatch):
         plan.dispatch(x, route)
 
 
+class _LibraryThatTakesEverything:
+    """Stands in for the library where only the numbers handed to it matter."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args[1]))
+            return _lib.MRS_OK
+
+        return call
+
+
+def test_dispatch_backward_takes_the_tokens_that_were_ordered(monkeypatch):
+    """Entries of row_of_slot behind the ordered tokens are not read as rows, whoever ordered how many before."""
+    from wgpu_morton_code_radix_sort_test_amd import api
+
+    monkeypatch.setattr(api, "_raw_stream", lambda index: 0)
+    captured = [False]
+    monkeypatch.setattr(api, "_capturing", lambda: captured[0])
+    plan = _plan_on_the_cpu(tokens=6)
+    plan.lib = _LibraryThatTakesEverything()
+    grad = torch.zeros(plan.max_rows, 5)
+    ids = torch.zeros(6, 2, dtype=torch.int32)
+
+    def took(route, **kw):
+        out = plan.dispatch_backward(grad, route, **kw)
+        assert plan.lib.calls[-1] == ("mrs_route_dispatch_backward", out.size(0))
+        return out.size(0)
+
+    route = plan.new_map()
+    assert took(route) == 6  # nothing known of it: all it holds
+    for tokens in (6, 2, 4, 6, 1, 0):
+        assert plan.order(ids[:tokens], route) is route
+        assert took(route) == tokens
+        assert took(route, tokens=3) == 3
+    with pytest.raises(ValueError, match="x_grad_out"):
+        plan.dispatch_backward(grad, route, x_grad_out=torch.zeros(6, 5))
+    assert took(plan.order(ids[:2])) == 2
+    # a map somebody else wrote, or a view of one, holds what it has room for
+    assert took(mrs.RouteMap(route.row_of_slot[:5], route.slot_of_row, route.counts, route.offsets)) == 5
+    # a refused ordering changes nothing
+    with pytest.raises(ValueError):
+        plan.order(ids.long(), route)
+    assert took(route) == 0
+    # captured orderings run again when nobody says so: the count stands as long as all agree on it
+    route, captured[0] = plan.new_map(), True
+    plan.order(ids[:3], route)
+    assert took(route) == 3
+    captured[0] = False
+    plan.order(ids[:3], route)
+    assert took(route) == 3
+    plan.order(ids[:4], route)
+    plan.order(ids[:3], route)
+    with pytest.raises(ValueError, match="tokens"):
+        plan.dispatch_backward(grad, route)
+    assert took(route, tokens=3) == 3
+
+
 @pytest.mark.parametrize("gate", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("normalize", [False, True])
 def test_derivative_formula_matches_differences(gate, normalize):

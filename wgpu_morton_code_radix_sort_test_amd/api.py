@@ -6,7 +6,8 @@ into libmrs.so.  Buffer roles follow the reference's `Buffers` struct
 `indices`/`indices_2` are payload A/B of `SortPlan.sort_pairs`.
 """
 import ctypes
-from dataclasses import dataclass
+from dataclasses import dataclass, field
+from typing import Optional
 
 import torch
 
@@ -409,18 +410,31 @@ _ROW_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _TYPE_8BIT = 3
 # The current stream's handle without the Stream object around it, which takes 3 us to make.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+_capturing = torch.cuda.is_current_stream_capturing
 
 
 @dataclass(frozen=True)
 class RouteMap:
     """`mrs_route_map`: int32 device tensors that say where every slot's row is.  `row_of_slot` [tokens,
     topk] holds a row or -1, `slot_of_row` [rows] a slot (token * topk + j) or -1, `counts` [experts] the rows an
-    expert has, `offsets` [experts + 1] where its segment starts and, last, where all of them end."""
+    expert has, `offsets` [experts + 1] where its segment starts and, last, where all of them end.  `tokens` is how many the last
+    `order` into this map had: entries of row_of_slot behind them say nothing.  None: no `order` was, all entries count."""
 
     row_of_slot: torch.Tensor
     slot_of_row: torch.Tensor
     counts: torch.Tensor
     offsets: torch.Tensor
+    tokens: Optional[int] = field(default=None, compare=False)
+    # a graph's replays write the map without a word here: once an ordering into it was captured, a second
+    # number of tokens makes `tokens` -1, not known, for good
+    _in_graph: bool = field(default=False, compare=False, repr=False)
+
+    def _ordered(self, tokens, capturing):
+        if (capturing or self._in_graph) and self.tokens is not None and self.tokens != tokens:
+            tokens = -1
+        object.__setattr__(self, "tokens", tokens)
+        if capturing:
+            object.__setattr__(self, "_in_graph", True)
 
 
 class RoutePlan:
@@ -587,13 +601,15 @@ class RoutePlan:
 
     def order(self, ids, map_out=None, stream=None):
         """`mrs_route_order`: a RouteMap of the slots sorted by ids [tokens, topk] (int32; ids outside [0, experts)
-        get no row).  Every tensor of `map_out` is written."""
+        get no row).  Every tensor of `map_out` is written, row_of_slot as far as the tokens go: what it holds behind them stays
+        and means nothing."""
         tokens = self._slots(ids, "ids")
         ids_ptr = self._per_slot(ids, "ids", tokens, torch.int32)
         if map_out is None:
             map_out = self.new_map(tokens, stream)
         raw, _ = self._map(map_out, tokens)
         _lib.check(self.lib.mrs_route_order(self._h, tokens, ids_ptr, raw, self._on_stream(stream)))
+        map_out._ordered(tokens, _capturing())
         return map_out
 
     def dispatch(self, x, route, rows_out=None, stream=None):
@@ -609,12 +625,16 @@ class RoutePlan:
         return rows_out
 
     def dispatch_backward(self, rows_grad, route, x_grad_out=None, tokens=None, stream=None):
-        """`mrs_route_dispatch_backward`: the gradient of x [tokens, hidden].  `tokens`: those that were ordered, where the map
-        has room for more (its own by default)."""
+        """`mrs_route_dispatch_backward`: the gradient of x [tokens, hidden], by default for the tokens of the last `order` into
+        this map.  Needed are they where orderings of different sizes share a map and one of them was captured into a graph."""
         kind = self._row_type(rows_grad, "rows_grad")
         hidden = rows_grad.size(1)
         if tokens is None:
-            tokens = route.row_of_slot.numel() // self.topk
+            tokens = route.tokens
+            if tokens is None:
+                tokens = route.row_of_slot.numel() // self.topk
+            elif tokens < 0:
+                raise ValueError("orderings of different sizes into this map, some of them in a graph: tokens has to be given")
         raw, rows = self._map(route, tokens)
         in_ptr, ld_in = self._rows(rows_grad, "rows_grad", rows, hidden, rows_grad.dtype)
         x_grad_out, out_ptr, ld_out = self._rows_out(x_grad_out, "x_grad_out", tokens, hidden, rows_grad.dtype, stream)
