@@ -528,7 +528,8 @@ int mrs_splitter_get(const mrs_splitter* sp, mrs_split_result* out);
  * graph; results do not depend on timing (no floating-point atomics).  Only mrs_route_order uses
  * memory of the handle: calls of it on one handle, and replays of graphs that hold one, must not
  * overlap in time, and the handle has to outlive such graphs.  Buffers need the alignment of their
- * element, nothing more; no output may overlap an input or another output. */
+ * element, nothing more; no output may overlap an input or another output.  The rows of a matrix are at
+ * most 2^40 elements apart and reach over at most 2^56 bytes. */
 typedef struct mrs_route mrs_route;
 
 #define MRS_GATE_SOFTMAX 0 /* p[e] = exp(s[e]) / sum of exp(s) over the experts that take part      */

@@ -65,3 +65,39 @@ def test_a_map_that_a_graph_writes_too(ctx, mrs):
     assert torch.equal(whole, plan.dispatch_backward(grad, plan.order(ids)))
     graph.replay()
     assert torch.equal(plan.dispatch_backward(grad, route, tokens=50), got)
+
+
+def test_matrices_beyond_the_address_range_are_refused(ctx, mrs):
+    """2^30 + 1 rows 2^40 floats apart: an extent of 2^72 bytes, which is 0 in 64 bits.  No slot has a row here, so that
+    no kernel would touch one."""
+    import ctypes
+
+    from wgpu_morton_code_radix_sort_test_amd import _lib
+
+    dev, lib, hidden, far = ctx.device, _lib.load_library(), 16, 1 << 40
+    plan = mrs.RoutePlan(ctx, 4, 4, 2)
+    none = torch.full((4, 2), -1, dtype=torch.int32, device=dev)
+    zeros = torch.zeros(5, dtype=torch.int32, device=dev)
+    x, buf, w = (torch.zeros(4, n, device=dev) for n in (hidden, hidden, 2))
+    sums = torch.zeros(4, 2, device=dev)
+    p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def calls(rows, ld):
+        m = ctypes.byref(_lib.RouteMapStruct(none.data_ptr(), None, zeros.data_ptr(), zeros.data_ptr(), rows))
+        f32 = 0
+        return [
+            lib.mrs_route_dispatch(plan._h, 4, m, f32, hidden, p(x), hidden, p(buf), ld, stream),
+            lib.mrs_route_dispatch_backward(plan._h, 4, m, f32, hidden, p(buf), ld, p(x), hidden, stream),
+            lib.mrs_route_combine(plan._h, 4, m, f32, hidden, p(buf), ld, p(w), p(x), hidden, stream),
+            lib.mrs_route_combine_backward(plan._h, 4, m, f32, hidden, p(x), hidden, p(buf), hidden, p(w), p(buf), ld, p(sums), stream),
+            lib.mrs_route_combine_backward(plan._h, 4, m, f32, hidden, p(x), hidden, p(buf), ld, p(w), p(buf), hidden, p(sums), stream),
+        ]
+
+    assert calls(4, hidden) == [_lib.MRS_OK] * 3 + [_lib.MRS_ERR_INVALID_ARGUMENT] * 2  # the last two: rows over rows_grad
+    assert "overlap" in lib.mrs_last_error_string().decode()
+    assert calls((1 << 30) + 1, far) == [_lib.MRS_ERR_INVALID_ARGUMENT] * 5
+    assert "2^56 bytes" in lib.mrs_last_error_string().decode()
+    assert calls((1 << 14) + 1, far) == [_lib.MRS_ERR_INVALID_ARGUMENT] * 5  # 2^56 + 64 bytes
+    torch.cuda.synchronize()
+    assert lib.mrs_route_destroy(None) == _lib.MRS_OK

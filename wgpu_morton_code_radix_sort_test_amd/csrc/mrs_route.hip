@@ -10,7 +10,8 @@ namespace {
 
 constexpr uint64_t kMaxRows = 0x7FFFFFFFull;       // row numbers are int32
 constexpr uint64_t kMaxHidden = 1ull << 24;        // column arithmetic in 32 bits
-constexpr uint64_t kMaxStride = 1ull << 40;        // row * stride stays far below 2^64
+constexpr uint64_t kMaxStride = 1ull << 40;        // stride * bytes of an element: 64-bit arithmetic has room
+constexpr uint64_t kMaxBytes = 1ull << 56;         // from a matrix's first byte to its last: so have row * stride and addresses
 
 int element_bytes(int32_t type) { return type == MRS_TYPE_F32 ? 4 : type == MRS_TYPE_8BIT ? 1 : 2; }
 
@@ -69,6 +70,9 @@ int check_matrix(const Matrix& m, const char* who, const char* name)
     if (m.stride < m.columns || m.stride > kMaxStride)
         return fail(MRS_ERR_INVALID_ARGUMENT, "%s: the rows of %s are %llu elements long but %llu apart", who, name,
                     (unsigned long long)m.columns, (unsigned long long)m.stride);
+    if (m.rows > 1 && m.stride > (kMaxBytes / m.bytes - m.columns) / (m.rows - 1))
+        return fail(MRS_ERR_INVALID_ARGUMENT, "%s: %s reaches over more than 2^56 bytes: %llu rows, %llu elements apart", who, name,
+                    (unsigned long long)m.rows, (unsigned long long)m.stride);
     return MRS_OK;
 }
 
