@@ -79,6 +79,25 @@ def test_bad_descriptions_are_refused(kw, word):
     assert word in _lib.load_library().mrs_last_error_string().decode()
 
 
+class _ContextOnTheCpu:
+    """Enough of a context for the checks before a handle is made."""
+
+    def __init__(self):
+        self.lib, self.device, self._h = _lib.load_library(), torch.device("cpu"), None
+
+
+@pytest.mark.parametrize("name", ["tokens", "experts", "topk", "align", "gate", "capacity"])
+def test_numbers_that_do_not_fit_their_field_are_refused(name):
+    """A field keeps the low bits of what it is given: 2^32 + 4 would go for 4."""
+    wide = 64 if name in ("tokens", "capacity") else 32
+    args = dict(tokens=8, experts=8, topk=2, align=1, capacity=0, gate=0)
+    with pytest.raises(mrs.MrsError, match="null argument"):  # right ones get as far as the missing context
+        mrs.RoutePlan(_ContextOnTheCpu(), **args)
+    for off in (1 << wide, -(1 << wide)):
+        with pytest.raises(ValueError, match=name):
+            mrs.RoutePlan(_ContextOnTheCpu(), **{**args, name: args[name] + off})
+
+
 def test_null_arguments_are_refused():
     lib = _lib.load_library()
     rows = ctypes.c_uint64()

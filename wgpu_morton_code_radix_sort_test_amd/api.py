@@ -450,9 +450,15 @@ class RoutePlan:
         self.ctx = ctx
         self.lib = ctx.lib
         self.device = ctx.device
+        # a ctypes field keeps the low bits of a number that does not fit
         for name, v in (("tokens", tokens), ("capacity", capacity)):
             if v < 0:
                 raise ValueError(f"{name} must not be negative")
+            if v >= 1 << 64:
+                raise ValueError(f"{name} = {v} does not fit 64 bits")
+        for name, v in (("experts", experts), ("topk", topk), ("align", align), ("gate", gate)):
+            if not -(1 << 31) <= v < 1 << 31:
+                raise ValueError(f"{name} = {v} does not fit 32 bits")
         self.desc = _lib.RouteDesc(tokens, experts, topk, align, gate, capacity, 1 if normalize else 0, scale)
         rows = ctypes.c_uint64()
         _lib.check(self.lib.mrs_route_max_rows(ctypes.byref(self.desc), ctypes.byref(rows)))
