@@ -136,7 +136,8 @@ int mrs_context_destroy(mrs_context* ctx);
  * librocprofiler-sdk-roctx.so or libroctx64.so) named as the reference names the pass it stands
  * for: "Morton Coding", "Histogram calculation", "Large Prefix Sum part 1", "Small Prefix Sum",
  * "Large Prefix Sum part 2", "Indexing"; launches without a counterpart there are named for what
- * they do ("Clear", "Local sort", "Gather", "Select", "Order", "Dispatch", "Combine").  `rocprofv3 --marker-trace --kernel-trace` then reads
+ * they do ("Clear", "Local sort", "Gather", "Select", "Order", "Dispatch", "Combine", and "Select backward",
+ * "Dispatch backward", "Combine backward").  `rocprofv3 --marker-trace --kernel-trace` then reads
  * like the reference's NSight capture.  Setting it fails with MRS_ERR_UNSUPPORTED if no roctx
  * library can be loaded. */
 #define MRS_ATTR_ROCTX_RANGES 4
@@ -604,8 +605,8 @@ int mrs_route_dispatch_backward(mrs_route* route, uint64_t tokens, const mrs_rou
 int mrs_route_combine(mrs_route* route, uint64_t tokens, const mrs_route_map* map, int32_t type, uint64_t hidden,
                       const void* rows_dev, uint64_t ld_rows, const float* weights_dev, void* out_dev, uint64_t ld_out,
                       void* stream);
-/* rows_grad[row_of_slot[t, j]] = weights[t, j] * out_grad[t] (rounded once; other rows as in
- * mrs_route_dispatch) and weights_grad[t, j] = sum over h of out_grad[t, h] * rows[row_of_slot[t, j], h] in
+/* rows_grad[row_of_slot[t, j]] = weights[t, j] * out_grad[t] (for 16-bit types rounded to 32 bits and
+ * then to the type, or at once; other rows as in mrs_route_dispatch) and weights_grad[t, j] = sum over h of out_grad[t, h] * rows[row_of_slot[t, j], h] in
  * 32 bits, 0 for a slot without a row. */
 int mrs_route_combine_backward(mrs_route* route, uint64_t tokens, const mrs_route_map* map, int32_t type, uint64_t hidden,
                                const void* out_grad_dev, uint64_t ld_out_grad, const void* rows_dev, uint64_t ld_rows,
