@@ -185,8 +185,8 @@ def test_dispatch_backward_takes_the_tokens_that_were_ordered(monkeypatch):
     """Entries of row_of_slot behind the ordered tokens are not read as rows, whoever ordered how many before."""
     from wgpu_morton_code_radix_sort_test_amd import api
 
-    monkeypatch.setattr(api, "_raw_stream", lambda index: 0)
     captured = [False]
+    monkeypatch.setattr(api, "_raw_stream", lambda index: 1 if captured[0] else 0)  # the null stream is never captured
     monkeypatch.setattr(api, "_capturing", lambda: captured[0])
     plan = _plan_on_the_cpu(tokens=6)
     plan.lib = _LibraryThatTakesEverything()

@@ -614,8 +614,12 @@ class RoutePlan:
         if map_out is None:
             map_out = self.new_map(tokens, stream)
         raw, _ = self._map(map_out, tokens)
-        _lib.check(self.lib.mrs_route_order(self._h, tokens, ids_ptr, raw, self._on_stream(stream)))
-        map_out._ordered(tokens, _capturing())
+        on = self._on_stream(stream)
+        _lib.check(self.lib.mrs_route_order(self._h, tokens, ids_ptr, raw, on))
+        # nothing is captured from the null stream; asking about others takes 0.3 us
+        capturing = on != 0 and _capturing()
+        if capturing or map_out.tokens != tokens:
+            map_out._ordered(tokens, capturing)
         return map_out
 
     def dispatch(self, x, route, rows_out=None, stream=None):
