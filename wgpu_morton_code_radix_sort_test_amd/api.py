@@ -443,7 +443,11 @@ class RoutePlan:
     order, `combine` brings them back weighted; the `*_backward` calls are the gradients.  An expert's rows start
     at a multiple of `align`; beyond `capacity` rows (0 = no limit) its later slots are dropped.  `gate`,
     `normalize` and `scale` say how scores become weights (include/mrs.h).  One handle runs one `order` at a time.
-    Nothing is recorded for autograd: a training step makes the backward calls itself."""
+    Nothing is recorded for autograd: a training step makes the backward calls itself.
+
+    Calls run on `stream` (the current one by default), and outputs they make belong to it.  As everywhere in torch, what a caller
+    hands over from another stream is the caller's to keep in order: `stream` has to wait for what writes an input, and the input's memory
+    must not be given back before the call has run (`Tensor.record_stream`, or a wait of the stream it was made on)."""
 
     def __init__(self, ctx, tokens, experts, topk, align=1, capacity=0, gate=GATE_SOFTMAX, normalize=True, scale=1.0):
         self._h = None

@@ -12,7 +12,7 @@
 // which counts all slots by itself (4096 slots 5.3 us, 16384 6.3, 32768 8.0, where two launches take 7.3, 7.9 and 7.9;
 // one workgroup alone 7.3 for 4096).  Above, a first launch counts tiles of 1, 2 or 4 slots a thread, and in a second one
 // every workgroup adds up the counts of the tiles before its own by itself (read from L2) instead of waiting for a scan
-// launch between the two (65536 slots 7.9 us, with four slots a thread 11.0).  2^20 slots: 17 us, 4 of them for the counts,
+// launch between the two (65536 slots 7.9 us, with four slots a thread 11.0).  2^20 slots: 16.7 us, 4 of them for the counts,
 // about 3 each for adding them up and for the writes to slot_of_row in runs of some 16 rows.
 #include <algorithm>
 
@@ -363,8 +363,10 @@ int launch_route_order(const OrderArgs& a, hipStream_t s)
         MRS_CHECK_LAUNCH("route_order_kernel");
         return MRS_OK;
     }
-    // Small tiles are ranked sooner, but every workgroup reads the counts of all of them: no more than 2^16 numbers, if that
-    // leaves 64 tiles (2^18 slots, 1024 experts: 256 tiles 20.7 us, 64 tiles 15.1).
+    // Small tiles are ranked sooner, but every workgroup reads the counts of all of them.  So threads take more slots, up to
+    // four, before tiles are more than `most`: 2^16 counts in all or 64 tiles (2^18 slots, 1024 experts: 256 tiles
+    // 20.7 us, 64 tiles 15.1).  From there on tiles do get more, up to kRouteMaxTiles: held at `most`, with several stretches
+    // each, 2^19 slots of 1024 experts take 23.1 us and not 20.2, 2^20 39 and not 30, of 512 23.3 and not 21.6.
     const uint64_t most = std::max(64u, std::min(kRouteMaxTiles, 65536u / a.experts));
     const uint32_t r = a.slots <= most * kThreads ? 1 : a.slots <= most * kThreads * 2 ? 2 : 4;
     const uint64_t tile = static_cast<uint64_t>(kThreads) * r;

@@ -16,8 +16,9 @@ constexpr uint32_t kShortThreads = 128;     // ... shorter than a wave's 64 vect
 constexpr uint32_t kMaxBlocks = 1u << 20;  // more work than that is looped over
 constexpr uint32_t kPadWaves = 2048;       // waves for the rows that fill segments up, two on a SIMD
 // combine's gradient: waves share a token's pieces evenly, but where that makes fewer waves than this, as many as there are pieces
-// for: 3 tokens of 6368 f32 (25 pieces) 36 -> 8.6 us, while
-// 3000 of 1109 (5 pieces) take 19 us evenly and 23 with four waves each.
+// for.  Evenly and with as many as that: 3 tokens of 4 slots and 6368 f32 (25 pieces) 17.7 and 6.0 us, 300 of 8 and 1500
+// bf16 (3 pieces) 13.7 and 11.2, 1000 of 4 and 2600 f32 (11 pieces) 24.2 and 18.8; but 3000 of 3 and 1109 f32 (5 pieces) 18.1 and
+// 22.6.  A bound of 512 takes the even way for the third, one of 8192 the other for the last.
 constexpr uint64_t kFewWaves = 2048;
 // Rows that cannot stay in the 256 MiB memory-side cache until somebody reads them again are streamed past the caches.
 constexpr uint64_t kStreamBytes = 256ull << 20;
@@ -145,7 +146,7 @@ __device__ __forceinline__ void load_weights(const float* __restrict__ weights, 
 
 // ---- dispatch: a row is read once and written `topk` times -----------------------------------
 // Workgroups of two waves, rows written through the caches: 0.239 ms for 16384 tokens, 8 slots, 4096 bf16 (1.1 GB
-// written, 5.3 TB/s in all; a plain copy reaches 5.0).  Larger workgroups or stores past the caches: 0.243 to 0.261; reading
+// written, 5.3 TB/s in all; plain copies reach 4.9 to 5.6).  Larger workgroups or stores past the caches: 0.243 to 0.261; reading
 // by row, so that the writes run through the buffer in order: 0.34, the reads no longer come from memory once.
 template <typename Elem, uint32_t K, bool WAVE>
 __global__ __launch_bounds__(kMoveThreads) void route_dispatch_kernel(const Elem* __restrict__ x, Elem* __restrict__ out,
@@ -191,9 +192,9 @@ __global__ __launch_bounds__(kMoveThreads) void route_dispatch_kernel(const Elem
 // workgroups of 4 waves 0.214, with ordinary loads 0.231, with neither 0.24.  Where the rows fit the memory-side
 // cache ordinary loads win: 64 MiB of them 13.5 against 14 us.
 template <typename T, uint32_t K, bool MORE, bool WEIGHTED, bool WAVE, bool STREAM>
-__global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_combine_kernel(const T* __restrict__ rows, T* __restrict__ out,
-                                                                    const int32_t* __restrict__ row_of_slot,
-                                                                    const float* __restrict__ weights, const MoveArgs a, const Cut c)
+__global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_combine_kernel(
+    const T* __restrict__ rows, T* __restrict__ out, const int32_t* __restrict__ row_of_slot, const float* __restrict__ weights,
+    const MoveArgs a, const Cut c)
 {
     constexpr uint32_t N = 16 / sizeof(T), THREADS = WAVE ? kSumThreads : kShortThreads;
     const uint32_t lane = threadIdx.x & ((1u << c.lanes_log2) - 1);
@@ -254,7 +255,7 @@ __global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_comb
 // product and the weighted piece written.  token_waves waves of a workgroup share a token; the lanes' partial dot
 // products are added by a fixed tree, the waves' in order, so results are the same every time.  Reads and writes
 // come in equal parts, past the caches where they are large: 0.445 ms for 16384 tokens, 8 slots, 4096 bf16 (5.3 TB/s; a
-// plain copy 5.0).  One wave for each token: 0.463; through the caches: 0.468.
+// plain copy 4.9 to 5.6).  One wave for each token: 0.463; through the caches: 0.468.
 
 // Sums of K values over a wave, M = 32.  While there are several values left, a step hands half of them to the
 // other half of the lanes.  Lane l returns the sum of value l / (64 / K).
@@ -280,11 +281,9 @@ __device__ __forceinline__ float sums_over_wave(const float (&v)[K])
 }
 
 template <typename T, uint32_t K, bool WAVE, bool STREAM>
-__global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_combine_backward_kernel(const T* __restrict__ rows, const T* __restrict__ out_grad,
-                                                                             T* __restrict__ rows_grad,
-                                                                             const int32_t* __restrict__ row_of_slot,
-                                                                             const float* __restrict__ weights, const MoveArgs a,
-                                                                             const Cut c)
+__global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_combine_backward_kernel(
+    const T* __restrict__ rows, const T* __restrict__ out_grad, T* __restrict__ rows_grad, const int32_t* __restrict__ row_of_slot,
+    const float* __restrict__ weights, const MoveArgs a, const Cut c)
 {
     constexpr uint32_t THREADS = WAVE ? kSumThreads : kShortThreads;
     if (blockIdx.x < c.pad_blocks) {
@@ -374,7 +373,7 @@ __global__ __launch_bounds__(WAVE ? kSumThreads : kShortThreads) void route_comb
                     half ^= 1;  // the next round writes the other half: one barrier a round is enough
                 }
             } else {
-for (uint32_t m = lanes >> 1; m > 0; m >>= 1)
+                for (uint32_t m = lanes >> 1; m > 0; m >>= 1)
 #pragma unroll
                     for (uint32_t j = 0; j < K; ++j) dot[j] += __shfl_xor(dot[j], static_cast<int>(m), static_cast<int>(lanes));
 #pragma unroll
@@ -430,11 +429,14 @@ int start_combine(const MoveArgs& a, hipStream_t s)
         const T* rows = static_cast<const T*>(a.rows_in);
         T* out = static_cast<T*>(a.token_out);
         if (c.lanes_log2 < 6)
-            hipLaunchKernelGGL((route_combine_kernel<T, K, MORE, WEIGHTED, false, false>), grid, block, 0, s, rows, out, a.row_of_slot, a.weights, a, c);
+            hipLaunchKernelGGL((route_combine_kernel<T, K, MORE, WEIGHTED, false, false>), grid, block, 0, s, rows, out, a.row_of_slot, a.weights,
+                               a, c);
         else if (!stream)
-            hipLaunchKernelGGL((route_combine_kernel<T, K, MORE, WEIGHTED, true, false>), grid, block, 0, s, rows, out, a.row_of_slot, a.weights, a, c);
+            hipLaunchKernelGGL((route_combine_kernel<T, K, MORE, WEIGHTED, true, false>), grid, block, 0, s, rows, out, a.row_of_slot, a.weights,
+                               a, c);
         else
-            hipLaunchKernelGGL((route_combine_kernel<T, K, MORE, WEIGHTED, true, true>), grid, block, 0, s, rows, out, a.row_of_slot, a.weights, a, c);
+            hipLaunchKernelGGL((route_combine_kernel<T, K, MORE, WEIGHTED, true, true>), grid, block, 0, s, rows, out, a.row_of_slot, a.weights,
+                               a, c);
     });
     MRS_CHECK_LAUNCH("route_combine_kernel");
     return MRS_OK;
@@ -453,11 +455,14 @@ int start_combine_backward(const MoveArgs& a, hipStream_t s)
         const T* grad = static_cast<const T*>(a.token_in);
         T* out = static_cast<T*>(a.rows_out);
         if (c.lanes_log2 < 6)
-            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, false, false>), grid, block, 0, s, rows, grad, out, a.row_of_slot, a.weights, a, c);
+            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, false, false>), grid, block, 0, s, rows, grad, out, a.row_of_slot, a.weights,
+                               a, c);
         else if (!stream)
-            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, true, false>), grid, block, 0, s, rows, grad, out, a.row_of_slot, a.weights, a, c);
+            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, true, false>), grid, block, 0, s, rows, grad, out, a.row_of_slot, a.weights,
+                               a, c);
         else
-            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, true, true>), grid, block, 0, s, rows, grad, out, a.row_of_slot, a.weights, a, c);
+            hipLaunchKernelGGL((route_combine_backward_kernel<T, K, true, true>), grid, block, 0, s, rows, grad, out, a.row_of_slot, a.weights,
+                               a, c);
     });
     MRS_CHECK_LAUNCH("route_combine_backward_kernel");
     return MRS_OK;
