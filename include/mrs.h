@@ -606,8 +606,9 @@ int mrs_route_combine(mrs_route* route, uint64_t tokens, const mrs_route_map* ma
                       const void* rows_dev, uint64_t ld_rows, const float* weights_dev, void* out_dev, uint64_t ld_out,
                       void* stream);
 /* rows_grad[row_of_slot[t, j]] = weights[t, j] * out_grad[t] (for 16-bit types rounded to 32 bits and
- * then to the type, or at once; other rows as in mrs_route_dispatch) and weights_grad[t, j] = sum over h of out_grad[t, h] * rows[row_of_slot[t, j], h] in
- * 32 bits, 0 for a slot without a row. */
+ * then to the type, or at once; other rows as in mrs_route_dispatch) and
+ * weights_grad[t, j] = sum over h of out_grad[t, h] * rows[row_of_slot[t, j], h] in 32 bits, 0 for a slot
+ * without a row. */
 int mrs_route_combine_backward(mrs_route* route, uint64_t tokens, const mrs_route_map* map, int32_t type, uint64_t hidden,
                                const void* out_grad_dev, uint64_t ld_out_grad, const void* rows_dev, uint64_t ld_rows,
                                const float* weights_dev, void* rows_grad_dev, uint64_t ld_rows_grad, float* weights_grad_dev,

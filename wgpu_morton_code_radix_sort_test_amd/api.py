@@ -639,8 +639,8 @@ class RoutePlan:
         return rows_out
 
     def dispatch_backward(self, rows_grad, route, x_grad_out=None, tokens=None, stream=None):
-        """`mrs_route_dispatch_backward`: the gradient of x [tokens, hidden], by default for the tokens of the last `order` into
-        this map.  Needed are they where orderings of different sizes share a map and one of them was captured into a graph."""
+        """`mrs_route_dispatch_backward`: the gradient of x [tokens, hidden].  `tokens` is by default that of the last `order` into
+        this map, and has to be given where orderings of different sizes share a map and one of them was captured into a graph."""
         kind = self._row_type(rows_grad, "rows_grad")
         hidden = rows_grad.size(1)
         if tokens is None:
